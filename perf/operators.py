@@ -178,7 +178,6 @@ def prepare(case, seed):
         st["ids"] = _popular(n, v, gen)
         st["ids"][torch.rand(n, generator=gen, device=dev) < 0.01] = -1  # items the catalogue has lost
         st["ref"] = -math.log(v) - 2.0 + 2.0 * torch.randn(n, generator=gen, device=dev)
-        st["ref"][st["ids"] < 0] = 0.0  # as the reference model's own log-probabilities are
         st["scale"], st["beta"], st["smooth"] = 1.0, 0.1, 0.05
     return st
 
