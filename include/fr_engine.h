@@ -995,7 +995,8 @@ int fr_rms_norm_bwd(const void* d_dy, int64_t lddy, const void* d_dh, int64_t ld
                     const float* d_rstd, void* d_dx, void* d_dw, void* d_workspace, int64_t workspace_bytes,
                     void* stream);
 /* logp[i] = z[i, ids[i]] - log sum_v exp z[i, v], z[i, v] = scale <H[i], W[v]>, over all n_items rows of W
- * (d <= 256), without storing z; 0 where ids[i] is outside [0, n_items).  For the backward (any may be NULL):
+ * (d <= 256), without storing z; +0 where ids[i] is outside [0, n_items), and there alone (an item's value is -0 or
+ * less, or NaN).  For the backward (any may be NULL):
  * d_lse2 [n] the row's log2 sum exp2; d_rest [n] = 1 - p[i, ids[i]], p = exp(z - lse); and (only with d_rest)
  * d_o [n, d] = sum_{v != ids[i]} p[i, v] W[v].  The table starts at a 16-byte boundary. */
 int64_t fr_item_logp_fwd_workspace(int64_t n, int64_t n_items, int d, int64_t ldw, int dtype, int with_o);
@@ -1014,7 +1015,8 @@ int fr_item_logp_bwd(const void* d_h, int64_t ldh, int64_t n, const void* d_w, i
 /* Paired log ratios: m_p = sum over [off[p], off[p+1]) of (logp - ref) - the same over
  * [off[pairs + p], off[pairs + p + 1]); *d_loss = mean_p [(1 - a) softplus(-beta m_p) + a softplus(beta m_p)],
  * a = smoothing.  d_offsets [2 pairs + 1], non-decreasing (bounds are clamped to [0, n]); d_ref may be NULL
- * (zeros).  d_pair_loss [pairs] is scratch; d_grad [n] = d loss / d logp, written in full (zeros outside the
+ * (zeros).  With d_ref a position whose logp is +0 (all bits zero: no target, as fr_item_logp_fwd has it) takes no
+ * part: neither value is added, whatever d_ref holds there (NaN included), and its gradient is 0.  d_pair_loss [pairs] is scratch; d_grad [n] = d loss / d logp, written in full (zeros outside the
  * lists). */
 int fr_preference_loss(const float* d_logp, const float* d_ref, const int64_t* d_offsets, int64_t pairs, int64_t n,
                        float beta, float smoothing, float* d_loss, float* d_pair_loss, float* d_grad, void* stream);

@@ -97,7 +97,8 @@ def item_log_probs(user_rows: torch.Tensor, item_table: torch.Tensor, items: tor
     """``log_softmax(scale * user_rows @ item_table.T)[i, items[i]]`` as fp32 [n], over ALL items, without the
     [n, items] score matrix in either direction.  user_rows [n, d] and item_table [I, d]: both fp32 or
     both bf16, d <= 256; scale > 0 (an inverse temperature).  A position whose item is outside [0, I) --
-    padding, say -1 -- has the value 0 and no gradient, whatever its row holds."""
+    padding, say -1 -- has the value +0 and no gradient, whatever its row holds; an item's value is -0 or
+    less, so that preference_loss can tell the two apart."""
     return _ext().item_log_probs(user_rows, item_table, items, scale)
 
 
@@ -110,6 +111,9 @@ def preference_loss(logp: torch.Tensor, ref_logp: torch.Tensor | None, offsets: 
         loss = mean_p [(1 - a) softplus(-beta m_p) + a softplus(beta m_p)],  a = label_smoothing
 
     ``ref_logp``: the frozen reference model's values (no gradient), None for a loss without reference.
+    A position whose logp is +0 (a positive zero: item_log_probs had no target there) is left out of its list:
+    the reference's value is not counted either, whatever it is (NaN included), and its gradient is 0.  Without a
+    reference it adds its 0 and nothing is to be left out.
     ``offsets``: int64 device tensor [2 P + 1], non-decreasing; empty lists are allowed, positions outside
     every list get no gradient.  Returns a 0-dim fp32 tensor."""
     return _ext().preference_loss(logp, ref_logp, offsets, beta, label_smoothing)

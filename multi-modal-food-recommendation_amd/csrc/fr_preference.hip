@@ -600,7 +600,8 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void finish_kernel(FinishArgs a)
   if (t) return;
   if (a.lse2) a.lse2[row] = l2;
   if (a.rest) a.rest[row] = others / total;
-  a.logp[row] = !real ? 0.f : z >= m ? -log1pf(others) : (z - l2) * 0.6931471805599453f;
+  const float lp = z >= m ? -log1pf(others) : (z - l2) * 0.6931471805599453f;
+  a.logp[row] = !real ? 0.f : lp >= 0.f ? -0.f : lp;  // +0 is the mark of a row without a target
 }
 
 // dH[row, :d] = a c ((1 - p) W[target] - o): zeros without a target
@@ -883,6 +884,10 @@ __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ par
 }
 
 // --------------------------------------------------------------------------- preference loss
+// A position without a target (item_logp_fwd's +0; a target's value is -0 or less) has no log ratio: whatever the
+// reference holds there takes no part.
+__device__ __forceinline__ bool lost(float logp, const float* ref) { return ref && __float_as_uint(logp) == 0u; }
+
 // One wave per pair: its margin, its share of the loss (returned), and the gradient of every list member's
 // logp for a unit upstream gradient (a list's members share it).
 __device__ __forceinline__ float pair_loss_of(const float* __restrict__ logp, const float* __restrict__ ref,
@@ -896,7 +901,8 @@ __device__ __forceinline__ float pair_loss_of(const float* __restrict__ logp, co
     lo[k] = min(max(off[p + k * pairs], (int64_t)0), n);
     hi[k] = min(max(off[p + k * pairs + 1], lo[k]), n);
     double v = 0.0;
-    for (int64_t i = lo[k] + lane; i < hi[k]; i += 64) v += (double)logp[i] - (ref ? (double)ref[i] : 0.0);
+    for (int64_t i = lo[k] + lane; i < hi[k]; i += 64)
+      if (!lost(logp[i], ref)) v += (double)logp[i] - (ref ? (double)ref[i] : 0.0);
     s += k ? -v : v;
   }
   s = group_sum_d<64>(s);
@@ -907,7 +913,7 @@ __device__ __forceinline__ float pair_loss_of(const float* __restrict__ logp, co
   const float g = beta / (float)pairs * (smooth * sig - (1.f - smooth) * sig_neg);
 #pragma unroll
   for (int k = 0; k < 2; ++k)
-    for (int64_t i = lo[k] + lane; i < hi[k]; i += 64) grad[i] = k ? -g : g;
+    for (int64_t i = lo[k] + lane; i < hi[k]; i += 64) grad[i] = lost(logp[i], ref) ? 0.f : k ? -g : g;
   return (1.f - smooth) * (fmaxf(-m, 0.f) + tail) + smooth * (fmaxf(m, 0.f) + tail);
 }
 

@@ -87,8 +87,10 @@ def item_log_probs_grad(h, w, ids, scale, up):
 
 
 def preference_loss(logp, ref, offsets, beta, smoothing):
+    """With a reference, a position whose logp is +0 has no target: it takes no part, whatever ref holds there."""
     pairs = (len(offsets) - 1) // 2
-    v = logp - (0.0 if ref is None else ref)
+    lost = (logp == 0) & ~np.signbit(logp) & (ref is not None)
+    v = np.where(lost, 0.0, logp - (0.0 if ref is None else ref))
     s = np.array([v[a:b].sum() for a, b in zip(offsets[:-1], offsets[1:])])
     m = beta * (s[:pairs] - s[pairs:])
     loss = ((1 - smoothing) * np.logaddexp(0, -m) + smoothing * np.logaddexp(0, m)).mean()
@@ -97,4 +99,5 @@ def preference_loss(logp, ref, offsets, beta, smoothing):
     for p in range(pairs):
         grad[offsets[p]:offsets[p + 1]] = slope[p]
         grad[offsets[pairs + p]:offsets[pairs + p + 1]] = -slope[p]
+    grad[lost] = 0.0
     return loss, grad
