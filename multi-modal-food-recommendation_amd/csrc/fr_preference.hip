@@ -277,6 +277,19 @@ __device__ __forceinline__ float other_half(float v) {
   return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
 }
 
+// A score in units of log 2.  Beyond fp32's range (|z| > 2.3e38) it is the range's end, so that a row of the type's
+// lowest values keeps its order; an infinite score stays one.
+__device__ __forceinline__ float in_log2(float s, float k) {
+  const float z = s * k;
+  return fabsf(s) < INFINITY ? fminf(fmaxf(z, -3.40282347e38f), 3.40282347e38f) : z;
+}
+
+// Up to this size of the reference (a maximum or a log-sum, in units of log 2) exponents are taken in one step,
+// exp2(s k - reference) with the product not rounded: its distance to the rounded reference is 2^-8 at most.  Beyond it
+// (a block of masked items, an outlying row) that distance is no longer small -- 2^75 at 1e30, and exp2 of it infinite --
+// so the product is rounded, too, as the reference was.
+constexpr float kLarge = 65536.f;
+
 __device__ __forceinline__ float max_or_nan(float a, float b) { return a != a ? a : b != b ? b : fmaxf(a, b); }
 
 // What a block of 32 rows has been multiplied by, undone: 2^-e of fp16 parts (1 without)
@@ -431,7 +444,7 @@ __global__ __launch_bounds__(256, waves_for(stats_regs<T, D, O>(NX))) void stats
 #pragma unroll
       for (int nb = 0; nb < NX; ++nb) {
         // tiny fp32 rows' scales may underflow together: not to 0, which times a masked -inf would be NaN
-        const float k = fmaxf(kx[nb] * ky, 1.17549435e-38f);
+        float k = fmaxf(kx[nb] * ky, 1.17549435e-38f);
         if (left < 32) {
 #pragma unroll
           for (int r = 0; r < 16; ++r)
@@ -442,31 +455,38 @@ __global__ __launch_bounds__(256, waves_for(stats_regs<T, D, O>(NX))) void stats
 #pragma unroll
           for (int r = 0; r < 16; ++r)
             if (result_row(r, 0) == at - 4 * half) {
-              target[nb] = s[nb][r] * k;
+              target[nb] = in_log2(s[nb][r], k);
               s[nb][r] = -INFINITY;
             }
         }
         float top = s[nb][0];
 #pragma unroll
         for (int r = 1; r < 16; ++r) top = fmaxf(top, s[nb][r]);
-        top *= k;
+        top = in_log2(top, k);
         if constexpr (O) {
           top = fmaxf(top, other_half(top));  // both halves' results meet in one product: one maximum
           if (__ballot(top > m[nb] + 8.f)) {
             const float m_new = fmaxf(m[nb], top), keep = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[nb] - m_new);
             m[nb] = m_new;
             sum[nb] *= keep;
+            // (what weighs nothing is dropped: items masked by the type's lowest value may have summed up to -inf)
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-              for (int r = 0; r < 16; ++r) acc[dt][r] *= keep;
+              for (int r = 0; r < 16; ++r) acc[dt][r] = keep == 0.f ? 0.f : acc[dt][r] * keep;
           }
         } else {
           const float m_new = fmaxf(m[nb], top);
           sum[nb] *= m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[nb] - m_new);
           m[nb] = m_new;
         }
-        const float base = m[nb] == -INFINITY ? 0.f : m[nb];  // nothing seen yet: exp2(-inf - 0) = 0
+        float base = m[nb] == -INFINITY ? 0.f : m[nb];  // nothing seen yet: exp2(-inf - 0) = 0
+        if (__ballot(!(fabsf(base) <= kLarge))) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[nb][r] = in_log2(s[nb][r], k) - base;
+          k = 1.f;
+          base = 0.f;
+        }
         float e = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -502,7 +522,8 @@ __global__ __launch_bounds__(256, waves_for(stats_regs<T, D, O>(NX))) void stats
   }
 }
 
-// The splits' statistics joined in their order, logp, lse (log 2 units) and, with O, o and 1 - p of the target.
+// The splits' statistics joined in their order, logp, lse (log 2 units, as a score and the logarithm of the sum beside
+// it: in one number the score could swallow the logarithm) and, with O, o and 1 - p of the target.
 // A group of D / 4 lanes per row, or (WIDE, for few rows of many splits) a workgroup per row, whose groups take
 // the splits in turn and are joined in group order.
 struct FinishArgs {
@@ -558,7 +579,9 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void finish_kernel(FinishArgs a)
       const float4 v = a.stats[q * a.n + row];
       const float w = __builtin_amdgcn_exp2f(v.x - base);
       sum = fmaf(v.y, w, sum);
-      o += *reinterpret_cast<const f32x4*>(a.part + (q * a.n + row) * D + t % L * 4) * w;
+      const f32x4 part = *reinterpret_cast<const f32x4*>(a.part + (q * a.n + row) * D + t % L * 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = w == 0.f ? o[j] : fmaf(part[j], w, o[j]);
     }
     if constexpr (WIDE) {
       red_o[g][t % L] = o;
@@ -590,7 +613,7 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void finish_kernel(FinishArgs a)
   const float top = fmaxf(m, z), low = top == -INFINITY ? 0.f : top;
   const float share = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - low);  // no other items: sum is 0 (or NaN)
   const float others = sum * share, total = others + __builtin_amdgcn_exp2f(z - low);
-  const float l2 = low + __builtin_log2f(total);
+  const float l2 = __builtin_log2f(total);
   if constexpr (O) {
     const float w = share / total;
 #pragma unroll
@@ -598,9 +621,12 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void finish_kernel(FinishArgs a)
       if (t * 4 + j < a.d) a.o[row * a.d + t * 4 + j] = o[j] * w;
   }
   if (t) return;
-  if (a.lse2) a.lse2[row] = l2;
+  if (a.lse2) {
+    a.lse2[row] = low;
+    a.lse2[a.n + row] = l2;
+  }
   if (a.rest) a.rest[row] = others / total;
-  const float lp = z >= m ? -log1pf(others) : (z - l2) * 0.6931471805599453f;
+  const float lp = z >= m ? -log1pf(others) : ((z - low) - l2) * 0.6931471805599453f;
   a.logp[row] = !real ? 0.f : lp >= 0.f ? -0.f : lp;  // +0 is the mark of a row without a target
 }
 
@@ -623,16 +649,17 @@ __global__ __launch_bounds__(256) void dh_kernel(const float* __restrict__ o, co
 // ------------------------------------------------------------------------------- operands
 // Rows as the kernels take them: parts of D columns, zeros behind the d-th.  With ids: a row without a target
 // (padding) is zero throughout, so that whatever it holds spreads neither into dW nor into the scale of the
-// rows around it.  For the gradients' users also, per row up to n_out: lse (+inf without a target: its
+// rows around it.  For the gradients' users also, per row up to n_out: lse in one number (+inf without a target: its
 // probabilities are 0; for bf16 -lse / (c log2 e), which the products are added to), the coefficient a_n c, the
-// target and its entry a_n c (1 - p).
+// target and its entry a_n c (1 - p); and inv is negative where one of the 32 has an lse beyond kLarge (or too large
+// for fp32 in the scores' units).
 template <typename T>
 struct Rows {
   const T* src;  // null: no rows
   int64_t ld, n, n_out;
   bool vec;
   bf16_t* out;  // [part][n_out][D]
-  float* inv;   // 2^-e per 32 rows, of fp16 parts
+  float* inv;   // per 32 rows 2^-e of fp16 parts, else 1
   const int64_t* ids;
   int64_t nv;
   const float *lse2, *rest, *up;
@@ -646,7 +673,7 @@ template <typename T, int D, bool GRAD>
 __global__ __launch_bounds__(256) void rows_kernel(Rows<T> h, Rows<T> w, int d) {
   using G = Geo<T, D, GRAD>;
   constexpr int TG = D >= 64 ? 256 : 128, K = 32 * G::CH / TG;
-  __shared__ uint32_t red[4];
+  __shared__ uint32_t red[4], red_large[4];
   const int64_t gh = h.src ? fr::ceil_div_dev(h.n_out, 32) : 0;
   const int64_t block = fr::block_number() * (256 / TG) + threadIdx.x / TG;
   const bool users = block < gh;
@@ -654,6 +681,7 @@ __global__ __launch_bounds__(256) void rows_kernel(Rows<T> h, Rows<T> w, int d) 
   const int64_t g = users ? block : block - gh;
   float v[K][8];
   uint32_t top = 0;
+  bool large = false;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int q = k * TG + threadIdx.x % TG, col = q % G::CH * 8;
@@ -679,23 +707,37 @@ __global__ __launch_bounds__(256) void rows_kernel(Rows<T> h, Rows<T> w, int d) 
       if (u < 0x7f800000u) top = max(top, u);  // the largest finite entry
     }
     if (a.coef && col == 0 && row < a.n_out) {
-      a.lse_o[row] = G::F32 ? (real ? a.lse2[row] : INFINITY) : real ? a.lse2[row] / (a.c * -kLog2e) : -INFINITY;
+      const float lse = real ? a.lse2[row] + a.lse2[a.n + row] : INFINITY;
+      const float start = G::F32 ? lse : real ? lse / (a.c * -kLog2e) : -INFINITY;
+      large |= real && !(fabsf(lse) <= kLarge && fabsf(start) < INFINITY);
+      a.lse_o[row] = start;
       a.coef[row] = real ? a.up[row] * a.c : 0.f;
       a.target[row] = real ? a.up[row] * a.c * a.rest[row] : 0.f;
       a.ids_o[row] = real ? (int32_t)id : -1;
     }
   }
-  float scale = 1.f;
-  if constexpr (G::HALF) {
+  float scale = 1.f, undo = 1.f;
+  if constexpr (G::HALF || GRAD) {
+    const bool any = __ballot(large);
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, 64));
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x / 64] = top;
+    if ((threadIdx.x & 63) == 0) {
+      red[threadIdx.x / 64] = top;
+      red_large[threadIdx.x / 64] = any;
+    }
     __syncthreads();
+    large = false;
 #pragma unroll
-    for (int i = 0; i < TG / 64; ++i) top = max(top, red[threadIdx.x / TG * (TG / 64) + i]);
-    const int e = top ? min(13 - ((int)(top >> 23) - 127), 120) : 0;  // largest in [2^13, 2^14), 2^e finite
-    scale = __uint_as_float((uint32_t)(e + 127) << 23);
-    if (a.src && threadIdx.x % TG == 0 && g * 32 < a.n_out) a.inv[g] = __uint_as_float((uint32_t)(127 - e) << 23);
+    for (int i = 0; i < TG / 64; ++i) {
+      top = max(top, red[threadIdx.x / TG * (TG / 64) + i]);
+      large |= red_large[threadIdx.x / TG * (TG / 64) + i] != 0;
+    }
+    if constexpr (G::HALF) {
+      const int e = top ? min(13 - ((int)(top >> 23) - 127), 120) : 0;  // largest in [2^13, 2^14), 2^e finite
+      scale = __uint_as_float((uint32_t)(e + 127) << 23);
+      undo = __uint_as_float((uint32_t)(127 - e) << 23);
+    }
+    if (a.src && threadIdx.x % TG == 0 && g * 32 < a.n_out) a.inv[g] = large ? -undo : undo;
   }
   if (!a.src) return;
 #pragma unroll
@@ -727,6 +769,7 @@ struct GradArgs {
   const float *inv_x, *inv_y;
   const float *lse, *coef, *target;  // per user, to a multiple of TY rows, plus 64
   const int32_t* ids;
+  const float *lse2, *lse2_sum;  // the forward's, [n] each
   float k;
   int64_t rt_n, sp_n, tiles_per_split;
   float* part;  // [split][nx][D], or null: one split, rows written to out
@@ -760,7 +803,7 @@ __global__ __launch_bounds__(256, waves_for(grad_regs<T, D>())) void grad_kernel
   const Stage<G> stage(a.Y, a.ldy, a.part_y, a.ny);
   float next = 1.f;
   const auto fetch = [&](int64_t t, int b) {
-    next = undo_tile<G>(a.inv_y, t, a.ny);
+    next = a.inv_y[t * G::SUBS + (threadIdx.x & 63) % G::SUBS];  // block q of the tile in lane q
     stage.load(t, tile[b]);
 #pragma unroll
     for (int q = 0; q < UR / 64; ++q) {
@@ -789,9 +832,11 @@ __global__ __launch_bounds__(256, waves_for(grad_regs<T, D>())) void grad_kernel
 #pragma unroll 1
     for (int sub = 0; sub < G::SUBS; ++sub) {
       if (t * G::TY + sub * 32 >= a.ny) break;
-      const float k = kx * undo_of<G>(inv, sub);
+      const float ky = lane_value(inv, sub);
+      const bool large = ky < 0.f;  // users whose lse is too large for one number
+      float k = G::F32 ? kx * fabsf(ky) : a.k;
       f32x16 s[1] = {};
-      if constexpr (!G::F32) {  // the products are added to -lse / k: their roundings at its size are below p's to bf16
+      if (!G::F32 && !large) {  // the products are added to -lse / k: their roundings at its size are below p's to bf16
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const f32x4 l = *reinterpret_cast<const f32x4*>(&u_lse[b][sub * 32 + 8 * q + 4 * half]);
@@ -802,10 +847,24 @@ __global__ __launch_bounds__(256, waves_for(grad_regs<T, D>())) void grad_kernel
       const int32_t uid = u_id[b][sub * 32 + (lane & 31)];
       scores<G, 1>(cur, sub, x, s);
       const bool hit = __ballot((uint32_t)uid - (uint32_t)x0 < 32u);  // a target of the tile is among the wave's items
+      if (large) {  // the exponents themselves, of users with an item (which are among the forward's n rows)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int u = sub * 32 + result_row(r, half);
+          float e = -INFINITY;
+          if (u_id[b][u] >= 0) {
+            const uint32_t at = (uint32_t)(t * G::TY) + u;
+            e = (in_log2(s[0][r], k) - a.lse2[at]) - a.lse2_sum[at];
+          }
+          s[0][r] = e;
+          __builtin_amdgcn_sched_barrier(0);  // a few values at a time
+        }
+        k = 1.f;
+      }
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         f32x4 l = {0.f, 0.f, 0.f, 0.f};
-        if constexpr (G::F32) l = *reinterpret_cast<const f32x4*>(&u_lse[b][sub * 32 + 8 * q + 4 * half]);
+        if (G::F32 && !large) l = *reinterpret_cast<const f32x4*>(&u_lse[b][sub * 32 + 8 * q + 4 * half]);
         const f32x4 c = *reinterpret_cast<const f32x4*>(&u_coef[b][sub * 32 + 8 * q + 4 * half]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -1217,6 +1276,8 @@ void logp_dw(const T* H, int64_t ldh, int64_t n, const T* W, int64_t ldw, int64_
   a.coef = w.coef;
   a.target = w.target;
   a.ids = w.ids;
+  a.lse2 = lse2;
+  a.lse2_sum = lse2 + n;
   a.k = c * kLog2e;
   a.rt_n = w.v.rt;
   a.sp_n = w.v.sp;

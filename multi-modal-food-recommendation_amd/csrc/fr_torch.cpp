@@ -378,7 +378,7 @@ LogP logp_run(const Tensor& h, const Tensor& w, const Tensor& ids, double scale,
   const int64_t n = h.size(0), d = h.size(1);
   LogP r;
   r.logp = at::empty({n}, f32);
-  if (for_dw) r.lse = at::empty({n}, f32);
+  if (for_dw) r.lse = at::empty({2, n}, f32);
   if (for_dh || for_dw) r.rest = at::empty({n}, f32);
   if (for_dh) r.o = at::empty({n, d}, f32);
   if (n) {

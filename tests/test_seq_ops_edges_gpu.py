@@ -1,5 +1,5 @@
 """The sequence operators on the GPU at the edges of their ranges: positions without a target beside a
-reference.  Tolerances as in test_seq_ops_gpu.py."""
+reference, masked and outlying rows.  Tolerances as in test_seq_ops_gpu.py."""
 import numpy as np
 import pytest
 import torch
@@ -97,3 +97,173 @@ def test_item_log_probs_of_targets_are_never_plus_zero(cuda, dt):
         for lp in (plain, ops.item_log_probs(H, W, ids)):
             assert torch.signbit(lp[real]).all()
             assert lp[3] == 0 and not torch.signbit(lp[3])
+
+
+# ------------------------------------------------------------------------ masked and outlying rows
+def own_bounds(H, W, ids, scale, up, t):
+    """logp_bounds of test_seq_ops_gpu.py, where a score's error is that of its own terms: d products (twice, see
+    there), 12 u of two 11-bit parts, and for fp32 2^-22 for what such parts leave of entries far below the largest of
+    their 32 rows; scores far below a row's log-sum have no part in it whatever their size.  exp2 gives 0 below 2^-126,
+    so a probability may be off by that much.  A score beyond fp32's range in units of log 2 is that range's end."""
+    n, d = H.shape
+    v = len(W)
+    ok = (ids >= 0) & (ids < v)
+    Hc, W = np.where(ok[:, None], H, 0.0), np.maximum(W, -1e300)  # -inf as a number: 0 times it is 0 in a row without target
+    with np.errstate(all="ignore"):
+        logp, z, lse = S.item_log_probs(Hc, W, ids, scale)
+        logp = np.where(logp < -1e200, -np.inf, np.maximum(logp, -np.log(2) * np.finfo(np.float32).max))
+        f32 = t == torch.float32
+        own = np.where(np.isfinite(z), np.abs(Hc) @ np.abs(W).T, 0.0)
+        dz = ((2 * (d + 2) + 12 * f32) * U * own + 2 * U * np.where(np.isfinite(z), np.abs(z), 0) / scale) * scale
+        dz += 2.0 ** -22 * f32
+        at = (np.arange(n), np.where(ok, ids, 0))
+        dzt, zt = dz[at], np.where(np.isfinite(z[at]), np.abs(z[at]), 0)
+        live = z + dz > lse[:, None] - 150
+        dz = np.where(live, dz, 0.0)
+        p = np.where(live, np.exp(z - lse[:, None]), 0.0)
+        top = np.maximum(np.abs(np.where(live, z, 0.0)).max(1), np.abs(lse))
+        dlse = 1.01 * (p * dz).sum(1) + (v / 2 + 100) * U + 6 * U * top
+        dlogp = np.where(ok, dzt + dlse + 4 * U * (top + zt), 0.0)
+        dH, dW, g = S.item_log_probs_grad(H, W, ids, scale, up)
+        c = np.where(ok, np.abs(up) * scale, 0.0)
+        e = 0.0 if f32 else e_of(t)
+        rel = dz + dlse[:, None] + 4 * U * (top[:, None] + 1) + 4 * U
+        dg = c[:, None] * (p * rel + 2.0 ** -126) + np.abs(g) * (4 * U + e)
+        tH = dg @ np.abs(W) + 2 * (v / 16 + 64) * U * np.abs(g) @ np.abs(W) + (e_of(t) + 4 * U) * np.abs(dH)
+        if not f32:
+            dg += c[:, None] * p * 2 * (d + 2) * U * np.abs(lse)[:, None]
+        tW = dg.T @ np.abs(Hc) + 2 * (n / 2 + 64) * U * np.abs(g).T @ np.abs(Hc) + (e_of(t) + 4 * U) * np.abs(dW)
+    return logp, dlogp, dH, tH, dW, tW
+
+
+def check_scores(ops, H, W, ids, t, scale=1.0, columns=None, upstream=1.0):
+    """Values without and with gradients and both gradients against float64 (the gradients' first `columns`)."""
+    n, v = len(H), len(W)
+    up = torch.linspace(-1, 1, n, device=H.device) * upstream
+    it = torch.from_numpy(ids).to(H.device)
+    want, tol, dH, tH, dW, tW = own_bounds(f64(H), f64(W), ids, scale, f64(up), t)
+    fin = np.isfinite(want)
+    for grad in (False, True):
+        with torch.set_grad_enabled(grad):
+            lp = ops.item_log_probs(H, W, it, scale)
+        assert (f64(lp)[~fin] == want[~fin]).all(), grad
+        close(f64(lp)[fin], want[fin], tol[fin], ("logp", grad))
+    gH, gW = torch.autograd.grad(lp, (H, W), up)
+    close(f64(gH)[:, :columns], dH[:, :columns], tH[:, :columns], "dH")
+    close(f64(gW), dW, tW, "dW")
+
+
+MASKS = [-1e4, -1e9, -1e30, "lowest"]
+
+
+@pytest.mark.parametrize("dt", ["bf16"])
+@pytest.mark.parametrize("d", [33, 64, 100, 256])
+@pytest.mark.parametrize("mask", MASKS)
+def test_item_log_probs_of_masked_items(cuda, mask, d, dt):
+    """Items taken out through a column that is 1 in every user row: their neighbours in the table keep their bits."""
+    from FoodRec.engine import ops
+    t = TYPES[dt]
+    value = torch.finfo(t).min if mask == "lowest" else mask
+    rng = np.random.default_rng(d)
+    n, v = 150, 333
+    s = 1.2 / d ** 0.25
+    H, W = randn(rng, (n, d), t, cuda, s), randn(rng, (v, d), t, cuda, s)
+    out = np.zeros(v, bool)
+    out[[0, 5, 31, 40, 331]] = True
+    out[96:170] = True  # whole blocks of rows, too
+    out[rng.integers(200, v, 12)] = True
+    H[:, -1] = 1.0
+    W[:, -1] = torch.where(torch.from_numpy(out).to(cuda), torch.tensor(value, dtype=t, device=cuda), torch.zeros((), dtype=t, device=cuda))
+    ids = rng.choice(np.flatnonzero(~out), n)
+    ids[:3] = 4, 6, 332  # beside masked rows
+    ids[9], ids[10], ids[11] = 5, -1, v  # a masked target, and none
+    with torch.no_grad():
+        H[10] = float("nan")
+    check_scores(ops, H.requires_grad_(), W.requires_grad_(), ids, t)
+
+
+@pytest.mark.parametrize("dt", ["bf16"])
+@pytest.mark.parametrize("d", [64, 100, 256])
+def test_item_log_probs_of_items_masked_by_the_users(cuda, d, dt):
+    """The other way round: the users' rows hold the mask's value, in a column that only masked items have."""
+    from FoodRec.engine import ops
+    t = TYPES[dt]
+    rng = np.random.default_rng(d + 1)
+    n, v = 150, 333
+    s = 1.2 / d ** 0.25
+    H, W = randn(rng, (n, d), t, cuda, s), randn(rng, (v, d), t, cuda, s)
+    out = torch.from_numpy(rng.random(v) < 0.1).to(cuda)
+    W[:, 3] = out.to(t)
+    for value in (-1e9, -1e30):
+        H[:, 3] = value
+        ids = rng.choice(np.flatnonzero(~out.cpu().numpy()), n)
+        check_scores(ops, H.clone().requires_grad_(), W.clone().requires_grad_(), ids, t)
+
+
+@pytest.mark.parametrize("dt", ["bf16"])
+@pytest.mark.parametrize("d", [64, 100])
+def test_item_log_probs_beside_an_outlying_user(cuda, d, dt):
+    """One user's row 1e12 times the others': its neighbours keep their bits, it is certain of one item."""
+    from FoodRec.engine import ops
+    t = TYPES[dt]
+    rng = np.random.default_rng(d + 2)
+    H, W = randn(rng, (150, d), t, cuda, 0.4), randn(rng, (333, d), t, cuda, 0.4)
+    H[37] *= 1e12
+    check_scores(ops, H.requires_grad_(), W.requires_grad_(), rng.integers(0, 333, 150), t)
+
+
+@pytest.mark.parametrize("dt", ["bf16"])
+@pytest.mark.parametrize("size", [3.0, 30.0])
+@pytest.mark.parametrize("d", [64, 256])
+def test_item_log_probs_of_large_scores(cuda, d, size, dt):
+    """Even rows whose scores are in the hundreds and thousands."""
+    from FoodRec.engine import ops
+    t = TYPES[dt]
+    rng = np.random.default_rng(d + 3)
+    H, W = randn(rng, (150, d), t, cuda, size), randn(rng, (333, d), t, cuda, size)
+    check_scores(ops, H.requires_grad_(), W.requires_grad_(), rng.integers(0, 333, 150), t)
+
+
+@pytest.mark.parametrize("dt", ["bf16"])
+@pytest.mark.parametrize("mask", [-1e30, "lowest"])
+@pytest.mark.parametrize("d,v", [(16, 50), (64, 700), (100, 1), (256, 300)])
+def test_item_log_probs_where_all_items_are_masked_alike(cuda, d, v, mask, dt):
+    """Every score of a row the same huge negative number: every item as likely as any other, in the gradients, too.
+    Roundings: the sum of v ones, one exp2 and log2; g rounded to the type, sums of n and of v products of it."""
+    from FoodRec.engine import ops
+    t = TYPES[dt]
+    rng = np.random.default_rng(d)
+    n = 130
+    H, W = torch.zeros(n, d, device=cuda, dtype=t), randn(rng, (v, d), t, cuda)
+    H[:, -1], W[:, -1] = 1.0, torch.finfo(t).min if mask == "lowest" else mask
+    H, W = H.requires_grad_(), W.requires_grad_()
+    ids = rng.integers(0, v, n)
+    ids[7] = -1
+    it, up = torch.from_numpy(ids).to(cuda), torch.linspace(-1, 1, n, device=cuda)
+    want = np.where(ids >= 0, -np.log(v), 0.0)
+    with torch.no_grad():
+        close(ops.item_log_probs(H, W, it), want, (v + 60) * U * (1 + np.log(v)))
+    lp = ops.item_log_probs(H, W, it)
+    close(lp, want, (v + 60) * U * (1 + np.log(v)))
+    gH, gW = torch.autograd.grad(lp, (H, W), up)
+    a, w = np.where(ids >= 0, f64(up), 0.0), f64(W)[:, :-1]
+    e = 0.0 if t == torch.float32 else e_of(t)
+    dH = a[:, None] * (w[ids] - w.mean(0))
+    size = np.abs(a)[:, None] * (np.abs(w[ids]) + np.abs(w).mean(0))
+    close(f64(gH)[:, :-1], dH, (e + (2 * v + 60) * U) * size + e_of(t) * np.abs(dH))
+    hit = np.zeros((v, n))
+    hit[ids, np.arange(n)] = 1.0
+    dW, size = (hit - 1 / v) @ a, (hit + 1 / v) @ np.abs(a)
+    close(f64(gW)[:, -1], dW, (e + (2 * v + 2 * n + 60) * U) * size + e_of(t) * np.abs(dW))
+    assert not gW[:, :-1].any()
+
+
+@pytest.mark.parametrize("dt", list(TYPES))
+@pytest.mark.parametrize("scale", [1e-38, 3e-36])
+def test_item_log_probs_of_vanishing_scale(cuda, scale, dt):
+    """A temperature so high that the log-sum in the scores' units leaves fp32's range."""
+    from FoodRec.engine import ops
+    t = TYPES[dt]
+    rng = np.random.default_rng(51)
+    H, W = randn(rng, (150, 64), t, cuda, 0.4), randn(rng, (700, 64), t, cuda, 0.4)
+    check_scores(ops, H.requires_grad_(), W.requires_grad_(), rng.integers(0, 700, 150), t, scale, upstream=1e30)
