@@ -1000,7 +1000,8 @@ int fr_rms_norm_bwd(const void* d_dy, int64_t lddy, const void* d_dh, int64_t ld
  * d_lse2 [2][n], whose sum is the row's log2 sum exp2 (a score, and what the sum adds to it); d_rest [n] = 1 - p[i, ids[i]], p = exp(z - lse); and (only with d_rest)
  * d_o [n, d] = sum_{v != ids[i]} p[i, v] W[v].  The table starts at a 16-byte boundary.  Masks by large negative
  * scores are taken at their value, up to the type's lowest (a row of nothing else is a uniform choice); scores beyond
- * +-2.3e38 (fp32's range in units of log 2) are that range's end. */
+ * +-2.3e38 (fp32's range in units of log 2) are that range's end.  A score of -inf is no choice (a row of nothing else
+ * has NaN), and an infinite entry's column of dH no number (0 times it). */
 int64_t fr_item_logp_fwd_workspace(int64_t n, int64_t n_items, int d, int64_t ldw, int dtype, int with_o);
 int fr_item_logp_fwd(const void* d_h, int64_t ldh, int64_t n, const void* d_w, int64_t ldw, int64_t n_items, int d,
                      int dtype, const int64_t* d_ids, float scale, float* d_logp, float* d_lse2, float* d_o,

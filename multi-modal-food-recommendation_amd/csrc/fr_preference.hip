@@ -223,6 +223,20 @@ __device__ __forceinline__ void load_x(const bf16_t* X, int64_t ld, int64_t part
     for (int kk = 0; kk < G::CH / 2; ++kk) f[p][kk] = *reinterpret_cast<const u32x4*>(row + p * part + kk * 16);
 }
 
+// an infinity or NaN among the wave's operands of bf16 parts
+template <int NS, int KK>
+__device__ __forceinline__ bool has_no_number(const u32x4 (&f)[NS][KK]) {
+  bool any = false;
+#pragma unroll
+  for (int p = 0; p < NS; ++p)
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        any |= (f[p][kk][j] & 0x7f80u) == 0x7f80u || (f[p][kk][j] & 0x7f800000u) == 0x7f800000u;
+  return __ballot(any);
+}
+
 template <bool HALF>
 __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 acc) {
   if constexpr (HALF)
@@ -626,7 +640,8 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void finish_kernel(FinishArgs a)
     a.lse2[a.n + row] = l2;
   }
   if (a.rest) a.rest[row] = others / total;
-  const float lp = z >= m ? -log1pf(others) : ((z - low) - l2) * 0.6931471805599453f;
+  // (an infinite score is no reference: NaN where it is +inf, or where the row has nothing but -inf)
+  const float lp = z >= m && fabsf(z) < INFINITY ? -log1pf(others) : ((z - low) - l2) * 0.6931471805599453f;
   a.logp[row] = !real ? 0.f : lp >= 0.f ? -0.f : lp;  // +0 is the mark of a row without a target
 }
 
@@ -652,14 +667,14 @@ __global__ __launch_bounds__(256) void dh_kernel(const float* __restrict__ o, co
 // rows around it.  For the gradients' users also, per row up to n_out: lse in one number (+inf without a target: its
 // probabilities are 0; for bf16 -lse / (c log2 e), which the products are added to), the coefficient a_n c, the
 // target and its entry a_n c (1 - p); and inv is negative where one of the 32 has an lse beyond kLarge (or too large
-// for fp32 in the scores' units).
+// for fp32 in the scores' units), for bf16 1/2 where one has no target.
 template <typename T>
 struct Rows {
   const T* src;  // null: no rows
   int64_t ld, n, n_out;
   bool vec;
   bf16_t* out;  // [part][n_out][D]
-  float* inv;   // per 32 rows 2^-e of fp16 parts, else 1
+  float* inv;   // per 32 rows 2^-e of fp16 parts, else 1 (and see above)
   const int64_t* ids;
   int64_t nv;
   const float *lse2, *rest, *up;
@@ -673,7 +688,7 @@ template <typename T, int D, bool GRAD>
 __global__ __launch_bounds__(256) void rows_kernel(Rows<T> h, Rows<T> w, int d) {
   using G = Geo<T, D, GRAD>;
   constexpr int TG = D >= 64 ? 256 : 128, K = 32 * G::CH / TG;
-  __shared__ uint32_t red[4], red_large[4];
+  __shared__ uint32_t red[4], red_kind[4];
   const int64_t gh = h.src ? fr::ceil_div_dev(h.n_out, 32) : 0;
   const int64_t block = fr::block_number() * (256 / TG) + threadIdx.x / TG;
   const bool users = block < gh;
@@ -681,7 +696,7 @@ __global__ __launch_bounds__(256) void rows_kernel(Rows<T> h, Rows<T> w, int d) 
   const int64_t g = users ? block : block - gh;
   float v[K][8];
   uint32_t top = 0;
-  bool large = false;
+  uint32_t kind = 0;  // 1: a user without a target, 2: one of a large lse
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int q = k * TG + threadIdx.x % TG, col = q % G::CH * 8;
@@ -709,7 +724,7 @@ __global__ __launch_bounds__(256) void rows_kernel(Rows<T> h, Rows<T> w, int d) 
     if (a.coef && col == 0 && row < a.n_out) {
       const float lse = real ? a.lse2[row] + a.lse2[a.n + row] : INFINITY;
       const float start = G::F32 ? lse : real ? lse / (a.c * -kLog2e) : -INFINITY;
-      large |= real && !(fabsf(lse) <= kLarge && fabsf(start) < INFINITY);
+      kind |= !real ? 1u : fabsf(lse) <= kLarge && fabsf(start) < INFINITY ? 0u : 2u;
       a.lse_o[row] = start;
       a.coef[row] = real ? a.up[row] * a.c : 0.f;
       a.target[row] = real ? a.up[row] * a.c * a.rest[row] : 0.f;
@@ -718,26 +733,27 @@ __global__ __launch_bounds__(256) void rows_kernel(Rows<T> h, Rows<T> w, int d) 
   }
   float scale = 1.f, undo = 1.f;
   if constexpr (G::HALF || GRAD) {
-    const bool any = __ballot(large);
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, 64));
+    for (int off = 32; off > 0; off >>= 1) {
+      top = max(top, (uint32_t)__shfl_xor((int)top, off, 64));
+      kind |= (uint32_t)__shfl_xor((int)kind, off, 64);
+    }
     if ((threadIdx.x & 63) == 0) {
       red[threadIdx.x / 64] = top;
-      red_large[threadIdx.x / 64] = any;
+      red_kind[threadIdx.x / 64] = kind;
     }
     __syncthreads();
-    large = false;
 #pragma unroll
     for (int i = 0; i < TG / 64; ++i) {
       top = max(top, red[threadIdx.x / TG * (TG / 64) + i]);
-      large |= red_large[threadIdx.x / TG * (TG / 64) + i] != 0;
+      kind |= red_kind[threadIdx.x / TG * (TG / 64) + i];
     }
     if constexpr (G::HALF) {
       const int e = top ? min(13 - ((int)(top >> 23) - 127), 120) : 0;  // largest in [2^13, 2^14), 2^e finite
       scale = __uint_as_float((uint32_t)(e + 127) << 23);
       undo = __uint_as_float((uint32_t)(127 - e) << 23);
     }
-    if (a.src && threadIdx.x % TG == 0 && g * 32 < a.n_out) a.inv[g] = large ? -undo : undo;
+    if (a.src && threadIdx.x % TG == 0 && g * 32 < a.n_out) a.inv[g] = kind & 2 ? -undo : !G::F32 && kind & 1 ? 0.5f : undo;
   }
   if (!a.src) return;
 #pragma unroll
@@ -794,6 +810,9 @@ __global__ __launch_bounds__(256, waves_for(grad_regs<T, D>())) void grad_kernel
   u32x4 x[1][G::NS][G::CH / 2];
   load_x<G>(a.X, a.ldx, a.part_x, a.nx, x0, x[0]);
   const float kx = a.k * undo<G>(a.inv_x, x0, a.nx);
+  // An infinite or NaN entry among the wave's items makes NaN of a zero row's score, so that blocks of users some of
+  // whom have no target (inv = 1/2) take the slower way, too.
+  const float slow = !G::F32 && has_no_number(x[0]) ? 1.f : 0.f;
   f32x16 acc[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
@@ -833,7 +852,7 @@ __global__ __launch_bounds__(256, waves_for(grad_regs<T, D>())) void grad_kernel
     for (int sub = 0; sub < G::SUBS; ++sub) {
       if (t * G::TY + sub * 32 >= a.ny) break;
       const float ky = lane_value(inv, sub);
-      const bool large = ky < 0.f;  // users whose lse is too large for one number
+      const bool large = ky < slow;  // negative: users whose lse is too large for one number
       float k = G::F32 ? kx * fabsf(ky) : a.k;
       f32x16 s[1] = {};
       if (!G::F32 && !large) {  // the products are added to -lse / k: their roundings at its size are below p's to bf16

@@ -153,7 +153,7 @@ def check_scores(ops, H, W, ids, t, scale=1.0, columns=None, upstream=1.0):
     close(f64(gW), dW, tW, "dW")
 
 
-MASKS = [-1e4, -1e9, -1e30, "lowest"]
+MASKS = [-1e4, -1e9, -1e30, "lowest", -np.inf]
 
 
 @pytest.mark.parametrize("dt", ["bf16"])
@@ -179,7 +179,8 @@ def test_item_log_probs_of_masked_items(cuda, mask, d, dt):
     ids[9], ids[10], ids[11] = 5, -1, v  # a masked target, and none
     with torch.no_grad():
         H[10] = float("nan")
-    check_scores(ops, H.requires_grad_(), W.requires_grad_(), ids, t)
+    # (0 times an infinite entry: dH has no number in its column)
+    check_scores(ops, H.requires_grad_(), W.requires_grad_(), ids, t, columns=d - 1 if mask == -np.inf else None)
 
 
 @pytest.mark.parametrize("dt", ["bf16"])
@@ -267,3 +268,25 @@ def test_item_log_probs_of_vanishing_scale(cuda, scale, dt):
     rng = np.random.default_rng(51)
     H, W = randn(rng, (150, 64), t, cuda, 0.4), randn(rng, (700, 64), t, cuda, 0.4)
     check_scores(ops, H.requires_grad_(), W.requires_grad_(), rng.integers(0, 700, 150), t, scale, upstream=1e30)
+
+
+@pytest.mark.parametrize("dt", ["bf16"])
+def test_item_log_probs_where_the_mask_leaves_nothing(cuda, dt):
+    """Every score -inf: there is no distribution, and the value is NaN, as log_softmax has it; other rows keep theirs."""
+    from FoodRec.engine import ops
+    t = TYPES[dt]
+    for d, v in ((16, 50), (100, 1), (64, 700)):
+        H, W = torch.ones(40, d, device=cuda, dtype=t), torch.zeros(v, d, device=cuda, dtype=t)
+        H[20:, 1] = 0.0
+        W[:, 1] = torch.finfo(t).min
+        H[:20, 1] = 4.0  # overflows to -inf; 0 in the others' rows leaves a score of 0
+        H, W = H.requires_grad_(), W.requires_grad_()
+        ids = torch.arange(40, device=cuda) % v
+        ids[4] = -1
+        with torch.no_grad():
+            plain = ops.item_log_probs(H, W, ids)
+        for lp in (plain, ops.item_log_probs(H, W, ids)):
+            assert lp[4] == 0
+            gone = torch.arange(20, device=cuda) != 4
+            assert torch.isnan(lp[:20][gone]).all()
+            close(lp[20:], np.full(20, -np.log(v)), 60 * U * (1 + np.log(v)))
