@@ -9,8 +9,8 @@ item_log_probs(H, W, ids)           infonce_loss,         log softmax over the w
                                     full_sort_topk        the score matrix, with both gradients
 preference_loss(logp, ref, off)     bpr_emb_loss          paired log ratios of lists of items
 
-Tables and rows are fp32 or bf16, arithmetic is fp32 (sums of a list's log-probabilities fp64), every
-stored value is rounded once.  All results are deterministic.  Calls are stream-ordered on the current
+Tables and rows are fp32 or bf16, arithmetic is fp32 (sums of a list's log-probabilities fp64; the matrix
+products of item_log_probs as it says), every stored value is rounded once.  All results are deterministic.  Calls are stream-ordered on the current
 stream of the tensors' device, never synchronise and may be captured into a HIP graph.  Each op is
 differentiable once.
 
@@ -96,7 +96,15 @@ def item_log_probs(user_rows: torch.Tensor, item_table: torch.Tensor, items: tor
                    scale: float = 1.0) -> torch.Tensor:
     """``log_softmax(scale * user_rows @ item_table.T)[i, items[i]]`` as fp32 [n], over ALL items, without the
     [n, items] score matrix in either direction.  user_rows [n, d] and item_table [I, d]: both fp32 or
-    both bf16, d <= 256; scale > 0 (an inverse temperature).  A position whose item is outside [0, I) --
+    both bf16, d <= 256; scale > 0 (an inverse temperature).
+
+    Products of fp32 rows are summed from 16-bit parts: a score keeps 2^-22 of the sum of its terms' sizes (fp32's own
+    order) and 2^-23 absolute, whatever rows lie beside it (blocks for which parts would not do go through fp32
+    instructions).  With bf16 rows the scores are exact products summed in fp32 (for the table's gradient added to the
+    row's log-sum, so rounded at its size), and the probabilities of the gradients' products are rounded to bf16, the
+    target's entry apart.  Items are masked by large negative scores or -inf; a row of nothing but -inf has NaN.
+
+    A position whose item is outside [0, I) --
     padding, say -1 -- has the value +0 and no gradient, whatever its row holds; an item's value is -0 or
     less, so that preference_loss can tell the two apart."""
     return _ext().item_log_probs(user_rows, item_table, items, scale)

@@ -28,14 +28,17 @@
 //
 //   scores   x = 2^-e (x0 + x1), two fp16 parts of 11 bits each, e shared by 32 rows so that their largest
 //            entry is in [2^13, 2^14): the products 00, 01, 10 leave 2^-22 of |x||y| (an fp32 sum of 64
-//            products leaves as much), and 2^-37 of the 32 rows' largest entry for those far below it
+//            products leaves as much), and 2^-38 of the 32 rows' largest entry for those far below it, which
+//            is kept below 2^-23 of a score by kPartsLimit
 //   g W, g H x = x0 + x1 + x2, three bf16 parts of 8 bits, which keep fp32's range (g spans many orders):
 //            the six products of parts down to 2^-18 of the largest; the dropped ones are below 2^-26
 //
 // which is 9 instructions of 32 x 32 x 16 per 16 columns of both products, instead of 16 fp32 ones of twice
 // the length.  From d = 65 on the five parts of a tile leave LDS for one workgroup per unit (or none), and the
-// scores that go with a second product are computed from its three bf16 parts, too.  (An infinite entry has
-// no such parts: its scores are NaN.)  For bf16 tables G is rounded to bf16 (2^-9 of each term, about the
+// scores that go with a second product are computed from its three bf16 parts, too.  Blocks whose rows differ too
+// much for the fp16 parts, with an infinite entry or one above 2^58 for the bf16 ones, get their scores from the fp32
+// rows on the fp32 instruction (7,168 x 45,630 x 64: pass 0.73 ms without such items, 1.1 with one in 1,000 masked by
+// -1e9, 1.3 with one in 100 = 28 % of the blocks, 1.9 where every block is one).  For bf16 tables G is rounded to bf16 (2^-9 of each term, about the
 // rounding of the result itself), but for the target's entry, which outweighs the others in dW: it is taken in two
 // parts (so is 1 - p, in fp32, in dH).  a_n and c are applied to g in dW and to the sum, in fp32, in dH.
 //
@@ -145,6 +148,29 @@ __device__ __forceinline__ void parts_of(const float (&v)[8], u32x4 (&out)[P]) {
         r[2 * j + 1] -= __uint_as_float(u & 0xffff0000u);
       }
     }
+}
+
+// the same of a row's entries as they come: one that would round to infinity is cut to the largest bf16 number, an
+// infinite one is in the first part alone
+template <int P>
+__device__ __forceinline__ void row_parts_of(const float (&v)[8], u32x4 (&out)[P]) {
+  if constexpr (P == 1) {
+    parts_of<1>(v, out);
+  } else {
+    float first[8], rest[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t u = __float_as_uint(v[j]), size = u & 0x7fffffffu;
+      first[j] = size >= 0x7f7f8000u && size <= 0x7f800000u ? __uint_as_float(u & 0xffff0000u) : v[j];
+      rest[j] = size == 0x7f800000u ? 0.f : v[j] - fr::to_f32(fr::from_f32<bf16_t>(first[j]));
+    }
+    u32x4 a[1], b[P - 1];
+    parts_of<1>(first, a);
+    parts_of<P - 1>(rest, b);
+    out[0] = a[0];
+#pragma unroll
+    for (int p = 1; p < P; ++p) out[p] = b[p - 1];
+  }
 }
 
 // eight values times `scale` as two vectors of fp16 parts
@@ -306,23 +332,75 @@ constexpr float kLarge = 65536.f;
 
 __device__ __forceinline__ float max_or_nan(float a, float b) { return a != a ? a : b != b ? b : fmaxf(a, b); }
 
-// What a block of 32 rows has been multiplied by, undone: 2^-e of fp16 parts (1 without)
+// fp32: what a block of 32 rows has been multiplied by, undone: 2^-e of fp16 parts, 1 of bf16 parts, +inf where its
+// entries have no such parts (0 behind the last row)
 template <typename G>
 __device__ __forceinline__ float undo(const float* inv, int64_t row, int64_t rows) {
-  if constexpr (G::HALF) return row < rows ? inv[row / 32] : 1.f;
+  if constexpr (G::F32) return row < rows ? inv[row / 32] : 0.f;
   else return 1.f;
 }
 
 // the same for the blocks of a tile, block q in lane q; read with undo_of
 template <typename G>
 __device__ __forceinline__ float undo_tile(const float* inv, int64_t t, int64_t rows) {
-  if constexpr (G::HALF) return inv[min(t * G::SUBS + (threadIdx.x & 63) % G::SUBS, fr::ceil_div_dev(rows, 32) - 1)];
+  if constexpr (G::F32) return inv[min(t * G::SUBS + (threadIdx.x & 63) % G::SUBS, fr::ceil_div_dev(rows, 32) - 1)];
   else return 1.f;
 }
 template <typename G>
 __device__ __forceinline__ float undo_of(float tile, int sub) {
-  if constexpr (G::HALF) return lane_value(tile, sub);
+  if constexpr (G::F32) return lane_value(tile, sub);
   else return 1.f;
+}
+
+// Two fp16 parts leave up to 2^-25 of an entry whose block has been brought below 2^14, however small the entry is: of
+// a score 2^-10 D k inv_x inv_y in all, in units of log 2, which the limit keeps below 2^-23 (a step of fp32 at 1).
+// Blocks beyond it -- an item masked by -1e9, a user row far above the table's -- would spoil the scores of the rows
+// beside the outlying one, and are computed from the fp32 rows.  Bf16 parts have fp32's range; there it is only blocks
+// with an entry above 2^58, whose products might not add up, or without a finite value.
+template <typename G>
+constexpr float kPartsLimit = G::HALF ? 0x1p-13f / (G::CH * 8) : 3.40282347e38f;
+
+// S = Y X^T of 32 rows each on the fp32 matrix instruction: an entry's products see that entry alone, infinities and NaN
+// are those of the plain formula.  y, x: this lane's rows of d columns, half h taking columns 8 i + 4 h .. + 4; y is
+// taken as zero where it is not real.  It waits for its loads (a pass of such blocks alone
+// takes 2.6 times as long).
+template <int NX>
+__device__ __forceinline__ void plain_scores(const float* y, bool real, const float* const (&x)[NX], int d,
+                                             f32x16 (&s)[NX]) {
+  struct alignas(4) Four {
+    float v[4];
+  };
+#pragma unroll
+  for (int nb = 0; nb < NX; ++nb) s[nb] = f32x16{};
+#pragma unroll 1
+  for (int c = 0; c < d; c += 8) {
+    const int at = c + (threadIdx.x & 32) / 8;
+    Four a = {}, b[NX] = {};
+    if (c + 8 <= d) {
+      a = *reinterpret_cast<const Four*>(y + at);
+#pragma unroll
+      for (int nb = 0; nb < NX; ++nb) b[nb] = *reinterpret_cast<const Four*>(x[nb] + at);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (at + j < d) {
+          a.v[j] = y[at + j];
+#pragma unroll
+          for (int nb = 0; nb < NX; ++nb) b[nb].v[j] = x[nb][at + j];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int nb = 0; nb < NX; ++nb)
+        s[nb] = __builtin_amdgcn_mfma_f32_32x32x2f32(real ? a.v[j] : 0.f, b[nb].v[j], s[nb], 0, 0, 0);
+  }
+}
+
+// a number that the compiler cannot tell from another: what is computed from it stays where it is used
+__device__ __forceinline__ int64_t here(int64_t v) {
+  asm volatile("" : "+v"(v));
+  return v;
 }
 
 // the A operand of the second product: Y columns dt * 32 .. + 32 for the 16 Y rows behind results 8 t .. 8 t + 8
@@ -398,6 +476,9 @@ struct StatsArgs {
   const bf16_t *H, *W;  // parts of rows of D columns, part_h / part_w elements apart
   int64_t ldh, part_h, n, ldw, part_w, nv;
   const float *inv_h, *inv_w;
+  const float *rows_h, *rows_w;  // fp32: the rows themselves, of d columns
+  int64_t ld_rows_h, ld_rows_w;
+  int d;
   const int64_t* ids;
   float k;
   int64_t rt_n, sp_n, tiles_per_split;
@@ -455,10 +536,23 @@ __global__ __launch_bounds__(256, waves_for(stats_regs<T, D, O>(NX))) void stats
       const float ky = undo_of<G>(inv, sub);
       f32x16 s[NX] = {};
       scores<G, NX>(cur, sub, x, s);
+      bool plain = false;
+      if constexpr (G::F32) {
+#pragma unroll
+        for (int nb = 0; nb < NX; ++nb) plain |= !(kx[nb] * ky <= kPartsLimit<G>);
+        plain = __ballot(plain);
+        if (plain) {
+          const float* rows[NX];
+#pragma unroll
+          for (int nb = 0; nb < NX; ++nb)
+            rows[nb] = a.rows_h + here(min(x0 + nb * 32 + (lane & 31), a.n - 1)) * a.ld_rows_h;
+          plain_scores<NX>(a.rows_w + here(min(y0 + (lane & 31), (int)a.nv - 1)) * a.ld_rows_w, true, rows, a.d, s);
+        }
+      }
 #pragma unroll
       for (int nb = 0; nb < NX; ++nb) {
-        // tiny fp32 rows' scales may underflow together: not to 0, which times a masked -inf would be NaN
-        float k = fmaxf(kx[nb] * ky, 1.17549435e-38f);
+        // tiny rows' scales may underflow together: not to 0, which times a masked -inf would be NaN
+        float k = plain ? a.k : G::HALF ? fmaxf(kx[nb] * ky, 1.17549435e-38f) : kx[nb] * ky;
         if (left < 32) {
 #pragma unroll
           for (int r = 0; r < 16; ++r)
@@ -667,7 +761,7 @@ __global__ __launch_bounds__(256) void dh_kernel(const float* __restrict__ o, co
 // rows around it.  For the gradients' users also, per row up to n_out: lse in one number (+inf without a target: its
 // probabilities are 0; for bf16 -lse / (c log2 e), which the products are added to), the coefficient a_n c, the
 // target and its entry a_n c (1 - p); and inv is negative where one of the 32 has an lse beyond kLarge (or too large
-// for fp32 in the scores' units), for bf16 1/2 where one has no target.
+// for fp32 in the scores' units; the block's lse are then 0 here), for bf16 1/2 where one has no target.
 template <typename T>
 struct Rows {
   const T* src;  // null: no rows
@@ -696,7 +790,7 @@ __global__ __launch_bounds__(256) void rows_kernel(Rows<T> h, Rows<T> w, int d) 
   const int64_t g = users ? block : block - gh;
   float v[K][8];
   uint32_t top = 0;
-  uint32_t kind = 0;  // 1: a user without a target, 2: one of a large lse
+  uint32_t kind = 0;  // 1: a user without a target, 2: one of a large lse, 4: an entry that is no number
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int q = k * TG + threadIdx.x % TG, col = q % G::CH * 8;
@@ -720,6 +814,7 @@ __global__ __launch_bounds__(256) void rows_kernel(Rows<T> h, Rows<T> w, int d) 
     for (int j = 0; j < 8; ++j) {
       const uint32_t u = __float_as_uint(v[k][j]) & 0x7fffffffu;
       if (u < 0x7f800000u) top = max(top, u);  // the largest finite entry
+      else kind |= 4u;
     }
     if (a.coef && col == 0 && row < a.n_out) {
       const float lse = real ? a.lse2[row] + a.lse2[a.n + row] : INFINITY;
@@ -732,7 +827,7 @@ __global__ __launch_bounds__(256) void rows_kernel(Rows<T> h, Rows<T> w, int d) 
     }
   }
   float scale = 1.f, undo = 1.f;
-  if constexpr (G::HALF || GRAD) {
+  if constexpr (G::F32 || GRAD) {
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) {
       top = max(top, (uint32_t)__shfl_xor((int)top, off, 64));
@@ -749,11 +844,21 @@ __global__ __launch_bounds__(256) void rows_kernel(Rows<T> h, Rows<T> w, int d) 
       kind |= red_kind[threadIdx.x / TG * (TG / 64) + i];
     }
     if constexpr (G::HALF) {
-      const int e = top ? min(13 - ((int)(top >> 23) - 127), 120) : 0;  // largest in [2^13, 2^14), 2^e finite
+      const int e = min(13 - ((int)(top >> 23) - 127), 120);  // largest in [2^13, 2^14), 2^e finite
       scale = __uint_as_float((uint32_t)(e + 127) << 23);
       undo = __uint_as_float((uint32_t)(127 - e) << 23);
     }
-    if (a.src && threadIdx.x % TG == 0 && g * 32 < a.n_out) a.inv[g] = kind & 2 ? -undo : !G::F32 && kind & 1 ? 0.5f : undo;
+    if (kind & 2) {  // the kernel takes these users' lse from the forward's two numbers
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int q = k * TG + threadIdx.x % TG;
+        const int64_t row = g * 32 + q / G::CH;
+        if (q % G::CH == 0 && row < a.n && a.ids_o[row] >= 0) a.lse_o[row] = 0.f;
+      }
+    }
+    if (G::F32 && (kind & 4 || (!G::HALF && top > 0x5c800000u /* 2^58 */))) undo = INFINITY;
+    if (a.src && threadIdx.x % TG == 0 && g * 32 < a.n_out)
+      a.inv[g] = kind & 2 ? -undo : !G::F32 && kind & 1 ? 0.5f : undo;
   }
   if (!a.src) return;
 #pragma unroll
@@ -771,7 +876,7 @@ __global__ __launch_bounds__(256) void rows_kernel(Rows<T> h, Rows<T> w, int d) 
     }
     if constexpr (GRAD || !G::HALF) {
       u32x4 o[G::NG];
-      parts_of<G::NG>(v[k], o);
+      row_parts_of<G::NG>(v[k], o);
 #pragma unroll
       for (int p = 0; p < G::NG; ++p) *reinterpret_cast<u32x4*>(out + (G::G0 + p) * part) = o[p];
     }
@@ -783,6 +888,8 @@ struct GradArgs {
   const bf16_t *X, *Y;  // rows of D columns, their parts part_x / part_y elements apart
   int64_t ldx, part_x, nx, ldy, part_y, ny;
   const float *inv_x, *inv_y;
+  const float *rows_x, *rows_y;  // fp32: the rows themselves, of d columns (users: the n that are there)
+  int64_t ld_rows_x, ld_rows_y, n;
   const float *lse, *coef, *target;  // per user, to a multiple of TY rows, plus 64
   const int32_t* ids;
   const float *lse2, *lse2_sum;  // the forward's, [n] each
@@ -821,8 +928,8 @@ __global__ __launch_bounds__(256, waves_for(grad_regs<T, D>())) void grad_kernel
 
   const Stage<G> stage(a.Y, a.ldy, a.part_y, a.ny);
   float next = 1.f;
-  const auto fetch = [&](int64_t t, int b) {
-    next = a.inv_y[t * G::SUBS + (threadIdx.x & 63) % G::SUBS];  // block q of the tile in lane q
+  const auto fetch = [&](int64_t t, int b, bool flags) {
+    if (flags) next = a.inv_y[t * G::SUBS + (threadIdx.x & 63) % G::SUBS];  // block q of the tile in lane q
     stage.load(t, tile[b]);
 #pragma unroll
     for (int q = 0; q < UR / 64; ++q) {
@@ -840,88 +947,112 @@ __global__ __launch_bounds__(256, waves_for(grad_regs<T, D>())) void grad_kernel
   };
 
   const int64_t t0 = sp * a.tiles_per_split, t1 = min(t0 + a.tiles_per_split, fr::ceil_div_dev(a.ny, G::TY));
-  if (t0 < t1) fetch(t0, 0);
-  for (int64_t t = t0; t < t1; ++t) {
-    wait_loads();
-    __syncthreads();
-    const float inv = next;
-    if (t + 1 < t1) fetch(t + 1, (int)(t + 1 - t0) & 1);
-    const int b = (int)(t - t0) & 1;
-    const uint32_t cur = lds_of(tile[b]);
-#pragma unroll 1
-    for (int sub = 0; sub < G::SUBS; ++sub) {
-      if (t * G::TY + sub * 32 >= a.ny) break;
-      const float ky = lane_value(inv, sub);
-      const bool large = ky < slow;  // negative: users whose lse is too large for one number
-      float k = G::F32 ? kx * fabsf(ky) : a.k;
-      f32x16 s[1] = {};
-      if (!G::F32 && !large) {  // the products are added to -lse / k: their roundings at its size are below p's to bf16
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const f32x4 l = *reinterpret_cast<const f32x4*>(&u_lse[b][sub * 32 + 8 * q + 4 * half]);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) s[0][4 * q + j] = l[j];
-        }
-      }
-      const int32_t uid = u_id[b][sub * 32 + (lane & 31)];
-      scores<G, 1>(cur, sub, x, s);
-      const bool hit = __ballot((uint32_t)uid - (uint32_t)x0 < 32u);  // a target of the tile is among the wave's items
-      if (large) {  // the exponents themselves, of users with an item (which are among the forward's n rows)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int u = sub * 32 + result_row(r, half);
-          float e = -INFINITY;
-          if (u_id[b][u] >= 0) {
-            const uint32_t at = (uint32_t)(t * G::TY) + u;
-            e = (in_log2(s[0][r], k) - a.lse2[at]) - a.lse2_sum[at];
+  const auto run = [&](auto f) {
+    constexpr bool FLAGS = decltype(f)::value;  // blocks of users are looked at one by one
+    if (t0 < t1) fetch(t0, 0, FLAGS);
+    for (int64_t t = t0; t < t1; ++t) {
+      wait_loads();
+      __syncthreads();
+      const float inv = next;
+      if (t + 1 < t1) fetch(t + 1, (int)(t + 1 - t0) & 1, FLAGS);
+      const int b = (int)(t - t0) & 1;
+      const uint32_t cur = lds_of(tile[b]);
+  #pragma unroll 1
+      for (int sub = 0; sub < G::SUBS; ++sub) {
+        if (t * G::TY + sub * 32 >= a.ny) break;
+        const float ky = FLAGS ? lane_value(inv, sub) : 1.f;
+        float k = G::F32 ? kx * fabsf(ky) : a.k;
+        const bool plain = G::F32 && __ballot(!(k <= kPartsLimit<G>));
+        const bool large = FLAGS && (ky < slow || plain);  // negative: users whose lse is too large for one number
+        if constexpr (G::HALF) k = fmaxf(k, 1.17549435e-38f);
+        f32x16 s[1] = {};
+        if constexpr (!G::F32) {  // the products are added to -lse / k: their roundings at its size are below p's to bf16
+  #pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const f32x4 l = *reinterpret_cast<const f32x4*>(&u_lse[b][sub * 32 + 8 * q + 4 * half]);
+  #pragma unroll
+            for (int j = 0; j < 4; ++j) s[0][4 * q + j] = l[j];
           }
-          s[0][r] = e;
-          __builtin_amdgcn_sched_barrier(0);  // a few values at a time
         }
-        k = 1.f;
-      }
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        f32x4 l = {0.f, 0.f, 0.f, 0.f};
-        if (G::F32 && !large) l = *reinterpret_cast<const f32x4*>(&u_lse[b][sub * 32 + 8 * q + 4 * half]);
-        const f32x4 c = *reinterpret_cast<const f32x4*>(&u_coef[b][sub * 32 + 8 * q + 4 * half]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float p = __builtin_amdgcn_exp2f(G::F32 ? fmaf(s[0][4 * q + j], k, -l[j]) : s[0][4 * q + j] * k);
-          s[0][4 * q + j] = -c[j] * p;
+        const int32_t uid = u_id[b][sub * 32 + (lane & 31)];
+        scores<G, 1>(cur, sub, x, s);
+        if (plain) {
+          const float* const rows[1] = {a.rows_x + here(min(xl, a.nx - 1)) * a.ld_rows_x};
+          const int64_t y = here(min(t * G::TY + sub * 32 + (lane & 31), a.n - 1));
+          plain_scores<1>(a.rows_y + y * a.ld_rows_y, uid >= 0, rows, a.d, s);
+          k = a.k;
         }
-      }
-      // the target's entry is a_n c (1 - p), from the forward's 1 - p
-      const auto targets = [&](auto&& put) {
-#pragma unroll
+        const bool hit = __ballot((uint32_t)uid - (uint32_t)x0 < 32u);  // a target of the tile is among the wave's items
+        if (large) {  // the exponents themselves, of users with an item (which are among the forward's n rows)
+  #pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int u = sub * 32 + result_row(r, half);
+            float e = -INFINITY;
+            if (u_id[b][u] >= 0) {
+              const uint32_t at = (uint32_t)(t * G::TY) + u;
+              e = in_log2(s[0][r], k);
+              if (ky < 0.f) e = (e - a.lse2[at]) - a.lse2_sum[at];
+            }
+            s[0][r] = e;
+            __builtin_amdgcn_sched_barrier(0);  // a few values at a time
+          }
+          k = 1.f;
+        }
+  #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const f32x4 v = *reinterpret_cast<const f32x4*>(&u_target[b][sub * 32 + 8 * q + 4 * half]);
-          const int4 id = *reinterpret_cast<const int4*>(&u_id[b][sub * 32 + 8 * q + 4 * half]);
-          put(4 * q, id.x == (int)xl, v[0]);
-          put(4 * q + 1, id.y == (int)xl, v[1]);
-          put(4 * q + 2, id.z == (int)xl, v[2]);
-          put(4 * q + 3, id.w == (int)xl, v[3]);
-          __builtin_amdgcn_sched_barrier(0);  // a few values at a time
+          f32x4 l = {0.f, 0.f, 0.f, 0.f};
+          if constexpr (G::F32) l = *reinterpret_cast<const f32x4*>(&u_lse[b][sub * 32 + 8 * q + 4 * half]);
+          const f32x4 c = *reinterpret_cast<const f32x4*>(&u_coef[b][sub * 32 + 8 * q + 4 * half]);
+  #pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float p = __builtin_amdgcn_exp2f(G::F32 ? fmaf(s[0][4 * q + j], k, -l[j]) : s[0][4 * q + j] * k);
+            s[0][4 * q + j] = -c[j] * p;
+          }
         }
-      };
-      if (hit) targets([&](int r, bool at, float v) { s[0][r] = at ? v : s[0][r]; });
-      u32x4 g[2][G::NG];
-      operand_of(s[0], g);
-      // bf16: what is left of the targets' entries in a second pass (the same code: the registers of one).  Without
-      // it dW is off by 0.0024-0.0025 of its norm, of few users by up to 0.004, with it by 0.0017, its own rounding;
-      // it costs nothing in 3,840 x 1M x 256 (6.5 ms) and 12-17 % of the pass where blocks of items are hit often
-      // (7,168 x 45,630 x 64 268 -> 316 us, 4,200 x 60,000 x 128 337 -> 391).
-      const int passes = hit && !G::F32 ? 2 : 1;
-#pragma unroll 1
-      for (int pass = 0; pass < passes; ++pass) {
-        if (pass) {
-          f32x16 r16;
-          targets([&](int r, bool at, float v) { r16[r] = at ? v - fr::to_f32(fr::from_f32<bf16_t>(v)) : 0.f; });
-          operand_of(r16, g);
+        // the target's entry is a_n c (1 - p), from the forward's 1 - p
+        const auto targets = [&](auto&& put) {
+  #pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(&u_target[b][sub * 32 + 8 * q + 4 * half]);
+            const int4 id = *reinterpret_cast<const int4*>(&u_id[b][sub * 32 + 8 * q + 4 * half]);
+            put(4 * q, id.x == (int)xl, v[0]);
+            put(4 * q + 1, id.y == (int)xl, v[1]);
+            put(4 * q + 2, id.z == (int)xl, v[2]);
+            put(4 * q + 3, id.w == (int)xl, v[3]);
+            __builtin_amdgcn_sched_barrier(0);  // a few values at a time
+          }
+        };
+        if (hit) targets([&](int r, bool at, float v) { s[0][r] = at ? v : s[0][r]; });
+        u32x4 g[2][G::NG];
+        operand_of(s[0], g);
+        // bf16: what is left of the targets' entries in a second pass (the same code: the registers of one).  Without
+        // it dW is off by 0.0024-0.0025 of its norm, of few users by up to 0.004, with it by 0.0017, its own rounding;
+        // it costs nothing in 3,840 x 1M x 256 (6.5 ms) and 12-17 % of the pass where blocks of items are hit often
+        // (7,168 x 45,630 x 64 268 -> 316 us, 4,200 x 60,000 x 128 337 -> 391).
+        const int passes = hit && !G::F32 ? 2 : 1;
+  #pragma unroll 1
+        for (int pass = 0; pass < passes; ++pass) {
+          if (pass) {
+            f32x16 r16;
+            targets([&](int r, bool at, float v) { r16[r] = at ? v - fr::to_f32(fr::from_f32<bf16_t>(v)) : 0.f; });
+            operand_of(r16, g);
+          }
+          accumulate<G, DT>(cur, sub, g, acc);
         }
-        accumulate<G, DT>(cur, sub, g, acc);
       }
     }
+  };
+  if constexpr (D < 256) {
+    run(std::true_type{});
+  } else {
+    // a loop of its own where none of the workgroup's blocks needs them (3,840 x 1M x 256 bf16 3.3 ms, 3.6 with the flags
+    // read and tested per tile; narrower ones have the registers)
+    static_assert(!G::HALF);
+    bool any = false;
+    for (int64_t i = t0 * G::SUBS + threadIdx.x; i < min(t1 * G::SUBS, a.ny / 32); i += 256)
+      any |= a.inv_y[i] < slow || !(kx * a.inv_y[i] <= kPartsLimit<G>);
+    if (__syncthreads_or(any)) run(std::true_type{});
+    else run(std::false_type{});
   }
   if (xl >= a.nx) return;
 #pragma unroll
@@ -1243,6 +1374,13 @@ void logp_fwd(const T* H, int64_t ldh, int64_t n, const T* W, int64_t ldw, int64
   a.nv = nv;
   a.inv_h = w.inv_h;
   a.inv_w = w.inv_w;
+  if constexpr (sizeof(T) == 4) {
+    a.rows_h = H;
+    a.rows_w = W;
+    a.ld_rows_h = ldh;
+    a.ld_rows_w = ldw;
+    a.d = d;
+  }
   a.ids = ids;
   a.k = c * kLog2e;
   a.rt_n = w.sp.rt;
@@ -1291,6 +1429,13 @@ void logp_dw(const T* H, int64_t ldh, int64_t n, const T* W, int64_t ldw, int64_
   a.part_y = w.n_pad * D;
   a.ny = w.n_pad;
   a.inv_y = w.inv_h;
+  if constexpr (sizeof(T) == 4) {
+    a.rows_x = W;
+    a.rows_y = H;
+    a.ld_rows_x = ldw;
+    a.ld_rows_y = ldh;
+    a.n = n;
+  }
   a.lse = w.lse;
   a.coef = w.coef;
   a.target = w.target;

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from oracle import seq as S
-from test_seq_ops_gpu import TYPES, U, close, e_of, f64, randn
+from test_seq_ops_gpu import TYPES, U, close, e_of, f64, randn, strided
 
 pytestmark = pytest.mark.gpu
 
@@ -156,7 +156,7 @@ def check_scores(ops, H, W, ids, t, scale=1.0, columns=None, upstream=1.0):
 MASKS = [-1e4, -1e9, -1e30, "lowest", -np.inf]
 
 
-@pytest.mark.parametrize("dt", ["bf16"])
+@pytest.mark.parametrize("dt", list(TYPES))
 @pytest.mark.parametrize("d", [33, 64, 100, 256])
 @pytest.mark.parametrize("mask", MASKS)
 def test_item_log_probs_of_masked_items(cuda, mask, d, dt):
@@ -183,7 +183,7 @@ def test_item_log_probs_of_masked_items(cuda, mask, d, dt):
     check_scores(ops, H.requires_grad_(), W.requires_grad_(), ids, t, columns=d - 1 if mask == -np.inf else None)
 
 
-@pytest.mark.parametrize("dt", ["bf16"])
+@pytest.mark.parametrize("dt", list(TYPES))
 @pytest.mark.parametrize("d", [64, 100, 256])
 def test_item_log_probs_of_items_masked_by_the_users(cuda, d, dt):
     """The other way round: the users' rows hold the mask's value, in a column that only masked items have."""
@@ -201,7 +201,7 @@ def test_item_log_probs_of_items_masked_by_the_users(cuda, d, dt):
         check_scores(ops, H.clone().requires_grad_(), W.clone().requires_grad_(), ids, t)
 
 
-@pytest.mark.parametrize("dt", ["bf16"])
+@pytest.mark.parametrize("dt", list(TYPES))
 @pytest.mark.parametrize("d", [64, 100])
 def test_item_log_probs_beside_an_outlying_user(cuda, d, dt):
     """One user's row 1e12 times the others': its neighbours keep their bits, it is certain of one item."""
@@ -213,7 +213,7 @@ def test_item_log_probs_beside_an_outlying_user(cuda, d, dt):
     check_scores(ops, H.requires_grad_(), W.requires_grad_(), rng.integers(0, 333, 150), t)
 
 
-@pytest.mark.parametrize("dt", ["bf16"])
+@pytest.mark.parametrize("dt", list(TYPES))
 @pytest.mark.parametrize("size", [3.0, 30.0])
 @pytest.mark.parametrize("d", [64, 256])
 def test_item_log_probs_of_large_scores(cuda, d, size, dt):
@@ -225,7 +225,7 @@ def test_item_log_probs_of_large_scores(cuda, d, size, dt):
     check_scores(ops, H.requires_grad_(), W.requires_grad_(), rng.integers(0, 333, 150), t)
 
 
-@pytest.mark.parametrize("dt", ["bf16"])
+@pytest.mark.parametrize("dt", list(TYPES))
 @pytest.mark.parametrize("mask", [-1e30, "lowest"])
 @pytest.mark.parametrize("d,v", [(16, 50), (64, 700), (100, 1), (256, 300)])
 def test_item_log_probs_where_all_items_are_masked_alike(cuda, d, v, mask, dt):
@@ -270,7 +270,7 @@ def test_item_log_probs_of_vanishing_scale(cuda, scale, dt):
     check_scores(ops, H.requires_grad_(), W.requires_grad_(), rng.integers(0, 700, 150), t, scale, upstream=1e30)
 
 
-@pytest.mark.parametrize("dt", ["bf16"])
+@pytest.mark.parametrize("dt", list(TYPES))
 def test_item_log_probs_where_the_mask_leaves_nothing(cuda, dt):
     """Every score -inf: there is no distribution, and the value is NaN, as log_softmax has it; other rows keep theirs."""
     from FoodRec.engine import ops
@@ -290,3 +290,22 @@ def test_item_log_probs_where_the_mask_leaves_nothing(cuda, dt):
             gone = torch.arange(20, device=cuda) != 4
             assert torch.isnan(lp[:20][gone]).all()
             close(lp[20:], np.full(20, -np.log(v)), 60 * U * (1 + np.log(v)))
+
+
+@pytest.mark.parametrize("dt", list(TYPES))
+@pytest.mark.parametrize("d", [50, 64])
+def test_item_log_probs_of_masked_items_layouts(cuda, d, dt):
+    """The same rows at any stride and alignment."""
+    from FoodRec.engine import ops
+    t = TYPES[dt]
+    rng = np.random.default_rng(d + 4)
+    H, W = randn(rng, (140, d), t, cuda, 0.4), randn(rng, (333, d), t, cuda, 0.4)
+    H[:, 0], W[:, 0] = 1.0, torch.where(torch.arange(333, device=cuda) % 9 == 2, -1e9, 0.0).to(t)
+    ids, up = torch.arange(140, device=cuda) * 9 % 333, torch.linspace(-1, 1, 140, device=cuda)
+
+    def both(h, w):
+        h, w = h.detach().requires_grad_(), w.detach().requires_grad_()
+        lp = ops.item_log_probs(h, w, ids)
+        return lp, *torch.autograd.grad(lp, (h, w), up)
+    for got in (both(strided(H), strided(W)), both(H.t().contiguous().t(), W.t().contiguous().t())):
+        assert all(torch.equal(a, b) for a, b in zip(got, both(H, W)))
