@@ -1123,7 +1123,8 @@ __device__ __forceinline__ float pair_loss_of(const float* __restrict__ logp, co
 #pragma unroll
   for (int k = 0; k < 2; ++k)
     for (int64_t i = lo[k] + lane; i < hi[k]; i += 64) grad[i] = lost(logp[i], ref) ? 0.f : k ? -g : g;
-  return (1.f - smooth) * (fmaxf(-m, 0.f) + tail) + smooth * (fmaxf(m, 0.f) + tail);
+  const float loss = (1.f - smooth) * (fmaxf(-m, 0.f) + tail);
+  return smooth > 0.f ? loss + smooth * (fmaxf(m, 0.f) + tail) : loss;  // not 0 times an infinite margin
 }
 
 // Few pairs: everything in one workgroup, the clearing of the gradient and the mean included

@@ -309,3 +309,24 @@ def test_item_log_probs_of_masked_items_layouts(cuda, d, dt):
         return lp, *torch.autograd.grad(lp, (h, w), up)
     for got in (both(strided(H), strided(W)), both(H.t().contiguous().t(), W.t().contiguous().t())):
         assert all(torch.equal(a, b) for a, b in zip(got, both(H, W)))
+
+
+@pytest.mark.parametrize("pairs", [2, 70])
+def test_preference_loss_of_infinite_margins(cuda, pairs):
+    """A rejected item that the policy cannot choose (logp -inf): no loss and no gradient without smoothing."""
+    from FoodRec.engine import ops
+    n = 2 * pairs
+    logp = torch.full((n,), -2.0, device=cuda)
+    logp[pairs] = -float("inf")
+    logp.requires_grad_()
+    off = torch.arange(n + 1, device=cuda)
+    loss = ops.preference_loss(logp, None, off, 0.5)
+    want = (pairs - 1) * np.log(2) / pairs
+    close(loss, want, 20 * U)
+    (g,) = torch.autograd.grad(loss, logp)
+    slope = np.full(pairs, -0.25 / pairs)
+    slope[0] = 0.0
+    close(g, np.concatenate([slope, -slope]), 20 * U)
+    assert ops.preference_loss(logp, None, off, 0.5, 0.1).item() == float("inf")
+    low = torch.tensor([-2.0, -float("inf"), -1.0], device=cuda).requires_grad_()
+    assert ops.preference_loss(low, None, torch.tensor([1, 2, 3], device=cuda), 0.5).item() == float("inf")
