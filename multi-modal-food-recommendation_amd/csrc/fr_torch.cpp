@@ -5,9 +5,11 @@
 // 512 x 64 dropout with its gradient takes 47 us through this binding and 74 us through a Python
 // autograd function over ctypes, of which 38 us are the autograd engine's own.  The C entry points
 // are called by address (bind()), so they are those of the one library that engine/native.py loaded.
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <cmath>
@@ -84,11 +86,21 @@ void on_gpu(const Tensor& t) {
          "); there is no CPU path");
 }
 
+// What a direct call of a kernel would lose in silence is refused: a tangent of forward-mode differentiation, and the
+// call itself in a trace, which would hold the allocation of its result alone.
+void plain_call(const char* name, const Tensor& t) {
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())
+    fail(name, ": engine operators have no forward-mode derivative");
+  if (torch::jit::tracer::isTracing()) fail(name, ": engine operators cannot be traced");
+}
+
 // the tensors on one GPU, the first in a supported type
 template <typename... O>
 void check(const char* name, const Tensor& t, const O&... others) {
+  plain_call(name, t);
   on_gpu(t);
   const auto same = [&](const Tensor& o) {
+    plain_call(name, o);
     on_gpu(o);
     if (o.device() != t.device()) fail(name, ": tensors on ", t.device(), " and ", o.device());
   };

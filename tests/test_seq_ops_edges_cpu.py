@@ -1,6 +1,7 @@
 """The edges of the sequence operators' ranges that need no GPU: the oracle there, and refusals."""
 import numpy as np
 import pytest
+import torch
 
 from oracle import seq as S
 
@@ -22,3 +23,43 @@ def test_preference_oracle_leaves_positions_without_a_target_out(smooth):
     a, _ = S.preference_loss(lp, None, off, 0.4, smooth)
     b, _ = S.preference_loss(np.where(lost, -0.0, lp), None, off, 0.4, smooth)
     assert a == b
+
+
+def _calls(ops, x, w, lp, i, c):
+    return {"embedding_scaled": lambda: ops.embedding_scaled(i, w, 2.0), "dropout": lambda: ops.dropout(x, 0.1, 1, c),
+            "rms_norm": lambda: ops.rms_norm(x), "add_rms_norm": lambda: ops.add_rms_norm(x, x),
+            "add_rms_norm_quant": lambda: ops.add_rms_norm_quant(x, x),
+            "item_log_probs": lambda: ops.item_log_probs(x, w, i),
+            "preference_loss": lambda: ops.preference_loss(lp, None, i)}
+
+
+def _inputs():
+    return (torch.zeros(3, 4), torch.zeros(5, 4), torch.zeros(3), torch.zeros(3, dtype=torch.int64),
+            torch.zeros(1, dtype=torch.int64))
+
+
+def test_forward_mode_is_refused():
+    """A tangent would be dropped: its primal asks for no gradient, so the kernels would be called directly."""
+    import torch.autograd.forward_ad as fwd
+    from FoodRec.engine import native, ops
+    x, w, lp, i, c = _inputs()
+    with fwd.dual_level():
+        dx, dw, dl = (fwd.make_dual(t, torch.ones_like(t)) for t in (x, w, lp))
+        for name, call in _calls(ops, dx, dw, dl, i, c).items():
+            with pytest.raises(native.EngineError, match=name + ".*forward-mode"):
+                call()
+        for call in (lambda: ops.item_log_probs(x, dw, i), lambda: ops.rms_norm(x, dx[0]),  # any argument's
+                     lambda: ops.dropout(x, 0.1, 1, c, residual=dx), lambda: ops.preference_loss(lp, dl, i)):
+            with pytest.raises(native.EngineError, match="forward-mode|GPU"):
+                call()
+        for name, call in _calls(ops, x, w, lp, i, c).items():  # without a tangent: the usual refusal of CPU tensors
+            with pytest.raises(native.EngineError, match="GPU"):
+                call()
+
+
+def test_tracing_is_refused():
+    from FoodRec.engine import native, ops
+    x, w, lp, i, c = _inputs()
+    for name in _calls(ops, x, w, lp, i, c):
+        with pytest.raises(native.EngineError, match=name + ".*traced"):
+            torch.jit.trace(lambda a, b, v: _calls(ops, a, b, v, i, c)[name](), (x, w, lp))

@@ -330,3 +330,24 @@ def test_preference_loss_of_infinite_margins(cuda, pairs):
     assert ops.preference_loss(logp, None, off, 0.5, 0.1).item() == float("inf")
     low = torch.tensor([-2.0, -float("inf"), -1.0], device=cuda).requires_grad_()
     assert ops.preference_loss(low, None, torch.tensor([1, 2, 3], device=cuda), 0.5).item() == float("inf")
+
+
+def test_forward_mode_and_traces_are_refused(cuda):
+    import torch.autograd.forward_ad as fwd
+    from FoodRec.engine import native, ops
+    x, w = torch.randn(6, 8, device=cuda), torch.randn(20, 8, device=cuda)
+    i, c = torch.arange(6, device=cuda), torch.zeros(1, dtype=torch.int64, device=cuda)
+    lp, off = torch.randn(6, device=cuda), torch.tensor([0, 3, 6], device=cuda)
+    with fwd.dual_level():
+        d = fwd.make_dual(x, torch.ones_like(x))
+        for call in (lambda: ops.embedding_scaled(i, fwd.make_dual(w, w), 2.0), lambda: ops.dropout(d, 0.1, 1, c),
+                     lambda: ops.dropout(x, 0.1, 1, c, residual=d), lambda: ops.rms_norm(d), lambda: ops.rms_norm(x, d[0]),
+                     lambda: ops.add_rms_norm(x, d), lambda: ops.add_rms_norm_quant(x, d),
+                     lambda: ops.item_log_probs(d, w, i), lambda: ops.item_log_probs(x, fwd.make_dual(w, w), i),
+                     lambda: ops.preference_loss(fwd.make_dual(lp, lp), None, off),
+                     lambda: ops.preference_loss(lp, fwd.make_dual(lp, lp), off)):
+            with pytest.raises(native.EngineError, match="forward-mode"):
+                call()
+        assert torch.equal(ops.rms_norm(x), ops.rms_norm(fwd.unpack_dual(d).primal))
+    with pytest.raises(native.EngineError, match="traced"):
+        torch.jit.trace(lambda a: ops.rms_norm(a), x)
