@@ -122,10 +122,34 @@ class Dropout(nn.Dropout):
     is stored for the backward and replays of a captured step draw new masks.  ``forward(x, residual)``
     adds the residual in the same pass.  Everything else (eval, host tensors, in-place, other types) is
     torch's own dropout.  A forward inside a backward pass (activation checkpointing) is refused: it would
-    draw another mask than the one whose result the loss was computed from."""
+    draw another mask than the one whose result the loss was computed from.  So is a first forward on a device
+    inside a graph capture: the counter would be made, and set to zero, by every replay.
+
+    The seed and the counter are no part of the state_dict; ``mask_state`` / ``load_mask_state`` carry them
+    over a checkpoint, without which a resumed run draws its first masks again."""
 
     def __getstate__(self):  # a copy of a layer in use draws masks of its own
         return {k: v for k, v in self.__dict__.items() if k != "_fr_dropout"}
+
+    def mask_state(self):
+        """{"seed", "step"} of the next mask (waits for the device), or None before the first one."""
+        state = self.__dict__.get("_fr_dropout")
+        if state is None:
+            return None
+        ops.settle_counter(state[1])
+        return {"seed": state[0], "step": int(state[1].item())}
+
+    def load_mask_state(self, state, device):
+        """Go on from ``mask_state`` of this or another layer, on ``device`` (None: from a seed of its own).  The
+        counter that captured graphs read is set in place; their seed is the one they were captured with."""
+        old = self.__dict__.pop("_fr_dropout", None)
+        if state is None:
+            return
+        counter = torch.full((1,), int(state["step"]), dtype=torch.int64, device=device)
+        if old is not None and old[1].device == counter.device:
+            ops.drop_pending(old[1])
+            counter = old[1].copy_(counter)
+        self.__dict__["_fr_dropout"] = (int(state["seed"]) & (2 ** 64 - 1), counter)
 
     def forward(self, x, residual=None):
         if (not self.training or self.inplace or not x.is_cuda or x.dtype not in (torch.float32, torch.bfloat16)):
@@ -136,12 +160,12 @@ class Dropout(nn.Dropout):
                                      "checkpointing): its mask follows a step counter; keep it outside")
         state = self.__dict__.get("_fr_dropout")
         if state is None or state[1].device != x.device:
-            salt = self.__dict__.get("_fr_salt")  # the layer's index in its model, if the model sets it
-            if salt is None:
-                global _LAYER_ORDINAL
-                _LAYER_ORDINAL += 1
-                salt = 1000 + _LAYER_ORDINAL
-            seed = (torch.initial_seed() * 0x9E3779B97F4A7C15 + salt + 1) & (2 ** 64 - 1)
+            if torch.cuda.is_current_stream_capturing():
+                raise native.EngineError("layers.Dropout: the first training forward on a device cannot be captured "
+                                         "(its step counter would be zeroed by every replay); run one before")
+            global _LAYER_ORDINAL
+            _LAYER_ORDINAL += 1
+            seed = (torch.initial_seed() * 0x9E3779B97F4A7C15 + 1001 + _LAYER_ORDINAL) & (2 ** 64 - 1)
             state = self.__dict__["_fr_dropout"] = (seed, torch.zeros(1, dtype=torch.int64, device=x.device))
         seed, counter = state
         ops.settle_counter(counter)  # a previous forward's increment not yet applied by a booked step

@@ -63,3 +63,51 @@ def test_tracing_is_refused():
     for name in _calls(ops, x, w, lp, i, c):
         with pytest.raises(native.EngineError, match=name + ".*traced"):
             torch.jit.trace(lambda a, b, v: _calls(ops, a, b, v, i, c)[name](), (x, w, lp))
+
+
+class _OnGpu:
+    """A stand-in for a device tensor, as far as layers.Dropout looks at one before any kernel."""
+    is_cuda, dtype, device = True, torch.float32, torch.device("cpu")
+
+
+def test_dropout_layer_refuses_its_first_forward_in_a_capture(monkeypatch):
+    """The counter would be zeroed by every replay.  With a counter made before, the forward goes on."""
+    from FoodRec.engine import layers, native, ops
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    seen = []
+    monkeypatch.setattr(ops, "dropout", lambda x, p, seed, counter, residual=None: seen.append((seed, int(counter))))
+    layer = layers.Dropout(0.5)
+    with pytest.raises(native.EngineError, match="cannot be captured"):
+        layer(_OnGpu())
+    assert "_fr_dropout" not in layer.__dict__
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    layer(_OnGpu())
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    layer(_OnGpu())
+    assert [s for _, s in seen] == [0, 1] and seen[0][0] == seen[1][0]
+
+
+def test_dropout_layer_mask_state(monkeypatch):
+    """A resumed layer goes on where the saved one stopped; copies, attributes set by a model or not, do not repeat it."""
+    import copy
+    from FoodRec.engine import layers, ops
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    seen = []
+    monkeypatch.setattr(ops, "dropout", lambda x, p, seed, counter, residual=None: seen.append((seed, int(counter))))
+    layer = layers.Dropout(0.5)
+    layer.__dict__["_fr_salt"] = 0
+    assert layer.mask_state() is None
+    for _ in range(3):
+        layer(_OnGpu())
+    state = layer.mask_state()
+    assert state == {"seed": seen[0][0], "step": 3}
+    copy.deepcopy(layer)(_OnGpu())
+    assert seen[-1][0] != state["seed"] and seen[-1][1] == 0
+    resumed = layers.Dropout(0.5)
+    resumed.load_mask_state(state, "cpu")
+    resumed(_OnGpu())
+    layer(_OnGpu())
+    assert seen[-1] == seen[-2] == (state["seed"], 3)
+    resumed.load_mask_state(None, "cpu")
+    resumed(_OnGpu())
+    assert seen[-1][0] != state["seed"]
