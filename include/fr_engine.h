@@ -981,7 +981,7 @@ int fr_dropout(const void* d_x, const void* d_residual, void* d_y, int64_t n, in
 /* h = x + residual (h = x without one), y = w h rstd, rstd = 1 / sqrt(mean(h^2) + eps) per row of d <= 8192.
  * y, h contiguous [rows, d]; d_h (only with a residual), d_rstd [rows] and d_w (ones) may be NULL; d_w is
  * fp32 or of the rows' type.  quant: y is written as e4m3 (fn) bytes of y / s, s = max |y| / 448 per row (1 for
- * a row of zeros) to d_scale [rows]. */
+ * a row of zeros; a subnormal s is rounded up, so that it is never 0 and |y| / s never above 448) to d_scale [rows]. */
 int fr_rms_norm_fwd(const void* d_x, int64_t ldx, const void* d_residual, int64_t ldr, int64_t rows, int d, int dtype,
                     const void* d_w, int w_dtype, float eps, void* d_y, int quant, float* d_scale, void* d_h,
                     float* d_rstd, void* stream);

@@ -58,6 +58,14 @@ __device__ __forceinline__ uint32_t gmax(uint32_t v, float* red) {
   return v;
 }
 
+// s of a row whose largest |y| has the bits `top`: never 0, and of the two subnormal numbers around a quotient the
+// one that keeps |y| / s within 8 bits' range
+__device__ __forceinline__ float quant_scale(uint32_t top) {
+  if (!top) return 1.f;
+  const float y = __uint_as_float(top), s = y / 448.f;
+  return s < 1.17549435e-38f && s * 448.f < y ? __uint_as_float(__float_as_uint(s) + 1u) : s;
+}
+
 struct FwdArgs {
   const void *x, *r, *w;
   void *y, *h;
@@ -130,7 +138,7 @@ __global__ __launch_bounds__(256) void rms_fwd_kernel(FwdArgs a) {
   }
   if constexpr (QUANT) {
     top = gmax<G>(top, red);
-    const float s = top ? __uint_as_float(top) / 448.f : 1.f;
+    const float s = quant_scale(top);
     if (live && t == 0) a.scale[row] = s;
     uint8_t* Q = static_cast<uint8_t*>(a.y) + row * a.d;
 #pragma unroll

@@ -351,3 +351,24 @@ def test_forward_mode_and_traces_are_refused(cuda):
         assert torch.equal(ops.rms_norm(x), ops.rms_norm(fwd.unpack_dual(d).primal))
     with pytest.raises(native.EngineError, match="traced"):
         torch.jit.trace(lambda a: ops.rms_norm(a), x)
+
+
+# ------------------------------------------------------------------------------- 8-bit norm
+@pytest.mark.parametrize("d", [64, 50, 2048])
+def test_add_rms_norm_quant_of_tiny_rows(cuda, d):
+    """Rows whose largest value is subnormal: the scale is still positive and no value leaves the 8 bits' range."""
+    from FoodRec.engine import ops
+    rng = np.random.default_rng(d)
+    tops = [2.0 ** -149, 3 * 2.0 ** -149, 447 * 2.0 ** -149, 671 * 2.0 ** -149, 449 * 2.0 ** -149, 1e-41, 1e-39, 1e-36]
+    x = torch.ones(len(tops), d, device=cuda)
+    w = torch.tensor(rng.uniform(-1, 1, (len(tops), d)), dtype=torch.float64)
+    w[:, 3] = 1.0
+    for k, top in enumerate(tops):
+        wk = (w[k] * top).float().to(cuda)
+        q, s, _ = ops.add_rms_norm_quant(x[k:k + 1], None, wk, 0.0)
+        y = f64(wk)  # rows of ones: rstd is 1 to rounding, and its step is far below one of a subnormal number
+        val = f64(q.float())[0] * f64(s)[0]
+        assert np.isfinite(val).all() and f64(s)[0] > 0
+        # s is rounded to a step of 2^-149 or up to the next; e4m3 as in test_add_rms_norm_quant
+        assert abs(f64(s)[0] - top / 448) <= 2.0 ** -149 + 64 * U * top / 448
+        assert (np.abs(val - y) <= (2.0 ** -4 + (d + 40) * U) * np.abs(y) + f64(s)[0] * 2.0 ** -10 + 2.0 ** -149).all()
