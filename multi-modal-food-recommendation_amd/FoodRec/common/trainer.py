@@ -20,10 +20,13 @@ attributes are swapped for HIP-backed Adjacency objects at construction.
 """
 from __future__ import annotations
 
+import contextlib
 import copy
+import gc
 import itertools
 import math
 import os
+import weakref
 from logging import getLogger
 from time import time
 
@@ -125,6 +128,22 @@ def book_step(parts, acc, nan_flag, accumulate=True):
 _CAPTURE_MODE = "thread_local"
 
 
+@contextlib.contextmanager
+def _capture(graph, pool=None):
+    """torch.cuda.graph with the garbage collector kept out: objects in reference cycles -- an older graph with its
+    trainer, whose destruction and memory pool's release are calls into the GPU runtime, or the autograd nodes that a
+    raised error's traceback holds -- go before the capture and not whenever a collection falls into it."""
+    gc.collect()
+    enabled = gc.isenabled()
+    gc.disable()
+    try:
+        with torch.cuda.graph(graph, pool=pool, capture_error_mode=_CAPTURE_MODE):
+            yield
+    finally:
+        if enabled:
+            gc.enable()
+
+
 class GraphedStep:
     """Trainer.train_step captured once in a HIP graph and replayed per batch.
 
@@ -170,7 +189,12 @@ class GraphedStep:
         if sampler.batch_size != self.B:
             raise ValueError("sampler batch size differs from the graphed step's")
         self.feed = sampler.device_feed()
-        self.feed.on_stage = self.flush  # pending steps read the epoch being replaced
+        flush = weakref.WeakMethod(self.flush)  # a feed does not keep the step (and its graphs) alive
+
+        def on_stage():  # pending steps read the epoch being replaced
+            if (f := flush()) is not None:
+                f()
+        self.feed.on_stage = on_stage
         return self.feed
 
     def flush(self):
@@ -246,7 +270,7 @@ class GraphedStep:
             self.gstate["acc"] = torch.zeros(self.n_parts, dtype=torch.float64, device=self.u.device)
             self.tr.optimizer.zero_grad()
             g = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(g, capture_error_mode=_CAPTURE_MODE):
+            with _capture(g):
                 self.static_loss = self._body(batch_idx, self.gstate, accumulate=True)
             self.graph = g
             self.captures += 1
@@ -260,7 +284,7 @@ class GraphedStep:
                 # the same body unroll times in one capture, sharing the one-step graph's memory pool
                 # (the two graphs replay in stream order)
                 gn = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(gn, pool=self.graph.pool(), capture_error_mode=_CAPTURE_MODE):
+                with _capture(gn, self.graph.pool()):
                     for k in range(self.unroll):
                         self.static_loss_n = self._body(batch_idx + k, self.gstate, accumulate=True)
                 self.graph_n = gn
@@ -411,18 +435,18 @@ class GraphedDPStep(GraphedStep):
             self.gstate["acc"] = torch.zeros(self.n_parts, dtype=torch.float64, device=self.u.device)
             tr.optimizer.zero_grad()
             ga = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(ga, capture_error_mode=_CAPTURE_MODE):
+            with _capture(ga):
                 self.static_loss = self._part_a(batch_idx, self.gstate, True)
             if self._split_b():
                 gb1, gb2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
-                with torch.cuda.graph(gb1, pool=ga.pool(), capture_error_mode=_CAPTURE_MODE):
+                with _capture(gb1, ga.pool()):
                     self._part_b1(self.gstate)
-                with torch.cuda.graph(gb2, pool=ga.pool(), capture_error_mode=_CAPTURE_MODE):
+                with _capture(gb2, ga.pool()):
                     self._part_b2(self.gstate)
                 self.graph_b = (gb1, gb2)
             else:
                 gb = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(gb, pool=ga.pool(), capture_error_mode=_CAPTURE_MODE):
+                with _capture(gb, ga.pool()):
                     self._part_b(self.gstate)
                 self.graph_b = (gb,)
             self.graph = ga
