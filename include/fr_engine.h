@@ -956,8 +956,8 @@ int fr_reg_combine_bwd(const float* d_g, int nb, float B, float w, float* d_da, 
 
 /* ------------------------------------------------------------------------------------------
  * Operators of models over item sequences: scaled embedding, dropout, residual RMS norm, item
- * log-probabilities and the preference loss.  dtype: FR_F32 or FR_BF16 storage, fp32 arithmetic,
- * one rounding per stored value; strides in elements, rows with unit stride inside.  Rows of any
+ * log-probabilities and the preference loss.  dtype: FR_F32 or FR_BF16 storage, fp32 arithmetic
+ * (fr_item_logp_*: matrix products of 16-bit parts, see there), one rounding per stored value; strides in elements, rows with unit stride inside.  Rows of any
  * width, stride and alignment are taken; 16-byte aligned rows of whole 16-byte words run faster.
  * Results depend on the inputs only, never on scheduling (no float atomics).
  * ------------------------------------------------------------------------------------------ */
@@ -1001,7 +1001,11 @@ int fr_rms_norm_bwd(const void* d_dy, int64_t lddy, const void* d_dh, int64_t ld
  * d_o [n, d] = sum_{v != ids[i]} p[i, v] W[v].  The table starts at a 16-byte boundary.  Masks by large negative
  * scores are taken at their value, up to the type's lowest (a row of nothing else is a uniform choice); scores beyond
  * +-2.3e38 (fp32's range in units of log 2) are that range's end.  A score of -inf is no choice (a row of nothing else
- * has NaN), and an infinite entry's column of dH no number (0 times it). */
+ * has NaN), and an infinite entry's column of dH no number (0 times it).
+ * Precision: fp32 rows are multiplied in 16-bit parts that leave 2^-22 of a score's terms and 2^-23 of a score at most
+ * (rows that differ too much for it go through fp32 instructions); bf16 rows exactly, with fp32 sums, which in dW are
+ * added to the row's log-sum (rounded at its size), and probabilities that both gradients' products take in bf16 (the
+ * target's entry in dW in two parts, in dH in fp32). */
 int64_t fr_item_logp_fwd_workspace(int64_t n, int64_t n_items, int d, int64_t ldw, int dtype, int with_o);
 int fr_item_logp_fwd(const void* d_h, int64_t ldh, int64_t n, const void* d_w, int64_t ldw, int64_t n_items, int d,
                      int dtype, const int64_t* d_ids, float scale, float* d_logp, float* d_lse2, float* d_o,

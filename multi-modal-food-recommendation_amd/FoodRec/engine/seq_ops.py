@@ -121,7 +121,8 @@ def preference_loss(logp: torch.Tensor, ref_logp: torch.Tensor | None, offsets: 
     ``ref_logp``: the frozen reference model's values (no gradient), None for a loss without reference.
     A position whose logp is +0 (a positive zero: item_log_probs had no target there) is left out of its list:
     the reference's value is not counted either, whatever it is (NaN included), and its gradient is 0.  Without a
-    reference it adds its 0 and nothing is to be left out.
+    reference it adds its 0 and nothing is to be left out.  (The mark is the policy's: where only the
+    reference had no target, its 0 counts as a value.)
     ``offsets``: int64 device tensor [2 P + 1], non-decreasing; empty lists are allowed, positions outside
     every list get no gradient.  Returns a 0-dim fp32 tensor."""
     return _ext().preference_loss(logp, ref_logp, offsets, beta, label_smoothing)

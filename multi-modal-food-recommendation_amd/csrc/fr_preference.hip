@@ -47,16 +47,18 @@
 // equally (no bank conflicts counted).  Tiles go from memory to LDS without registers, two in turn, one
 // barrier per tile.
 //
-// Bound by the matrix cores at the clock that their power allows (1.75-1.9 GHz under load; a library product of
-// 8192^3 in bf16 reaches 1,206 TFLOP/s): 3,840 x 1M x 256 bf16 statistics and o 3.15-3.25 ms (1,210-1,250 TFLOP/s), dW
-// 3.25-3.4 ms (1,160-1,210); 7,168 x 45,630 x 64 fp32 0.34-0.36 and 0.35-0.39 ms (statistics, dH and dW were 0.45, 0.90
-// and 0.87 with fp32 instructions).  Statistics alone are bound by the vector work per score (exponential,
-// multiply-add, sum, maximum: some 44 cycles per 64 scores, 32 of d = 128's products): 7,168 x 45,630 x 64 bf16 75-83 us;
-// 1,800 x 29,943 x 128 bf16 27 us, some 8 of them the start and the operands' loading.  The matrix cores are busy
-// 55-62 % of the cycles; what helped beside the products was fewer instructions and registers around them (addresses
-// as constants, -lse as the accumulators' start); reading further ahead, more tiles in flight, one block's scores
-// computed beside the statistics of another, no scheduling fences and wave priorities changed nothing beyond 2 %
-// or cost time.
+// Bound by the matrix cores at the clock that their power allows (1.7-1.9 GHz under load; a library product of
+// 8192^3 in bf16 reaches 1,206 TFLOP/s).  Medians of 20 launches each under a kernel trace: 3,840 x 1M x 256 bf16
+// statistics and o 3.24 ms (1,210 TFLOP/s), dW 3.31 ms (1,190), boxes differ by 5 %; 7,168 x 45,630 x 64 fp32 343 and
+// 363 us (statistics, dH and dW took 0.45, 0.90 and 0.87 ms with fp32 instructions).  Statistics alone are bound by the
+// vector work per score (exponential, multiply-add, sum, maximum: some 44 cycles per 64 scores, 32 of d = 128's
+// products): 1,800 x 29,943 x 128 bf16 28 us, some 8 of them the start and the operands' loading; a call of 7,168 x
+// 45,630 x 64 bf16 75 us.  The matrix cores are busy 53-60 % of the cycles; what helped beside the products was fewer
+// instructions and registers around them (addresses as constants, -lse as the accumulators' start); reading further
+// ahead, more tiles in flight, one block's scores computed beside the statistics of another, no scheduling fences and
+// wave priorities changed nothing beyond 2 % or cost time.
+// What is spilled with d = 256 (and d = 128 in fp32) is reloaded per tile or before the loops: 11 registers per tile of
+// 32 rows in bf16 with o, 5 in dW; fp32 10 with o, and 2 in dW of d = 128.
 #include "fr_vec.h"
 
 #include <algorithm>
@@ -273,8 +275,8 @@ __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 acc) {
 }
 
 // N steps of products whose A operands come from LDS, read AHEAD steps before their use: a read takes about
-// 128 cycles, a step 32 per product.  (d = 256 in bf16 has registers for two steps: with three, operands are
-// reloaded from scratch for every 32 rows, 7.17 -> 6.73 ms for the pass of 3,840 x 1M.)  The fences keep the
+// 128 cycles, a step 32 per product.  (d = 256 in bf16 has registers for two steps: with three, operands, too, are
+// reloaded from scratch for every 32 rows; two instead of three took the pass of 3,840 x 1M from 7.17 to 6.73 ms.)  The fences keep the
 // compiler from reading further ahead, which would spill the accumulators.
 template <int N, int P, typename L, typename M>
 __device__ __forceinline__ void pipelined(L&& load, M&& multiply) {
@@ -1027,8 +1029,8 @@ __global__ __launch_bounds__(256, waves_for(grad_regs<T, D>())) void grad_kernel
         operand_of(s[0], g);
         // bf16: what is left of the targets' entries in a second pass (the same code: the registers of one).  Without
         // it dW is off by 0.0024-0.0025 of its norm, of few users by up to 0.004, with it by 0.0017, its own rounding;
-        // it costs nothing in 3,840 x 1M x 256 (6.5 ms) and 12-17 % of the pass where blocks of items are hit often
-        // (7,168 x 45,630 x 64 268 -> 316 us, 4,200 x 60,000 x 128 337 -> 391).
+        // it costs nothing in 3,840 x 1M x 256 (6.7 ms) and 13-21 % of the pass where blocks of items are hit often
+        // (7,168 x 45,630 x 64 256 -> 309 us, 4,200 x 60,000 x 128 320 -> 385, 1,000 x 60,000 x 64 82 -> 97).
         const int passes = hit && !G::F32 ? 2 : 1;
   #pragma unroll 1
         for (int pass = 0; pass < passes; ++pass) {

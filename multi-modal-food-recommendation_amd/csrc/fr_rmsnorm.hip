@@ -9,8 +9,8 @@
 // per thread), so x and the residual are read once and y and h written once; the backward reads dy,
 // dh and h once.  A stored h of bf16 is rounded, which dw would show (each of its terms off by 2^-9, as
 // much as dw's own rounding): the backward then takes x and the residual and adds them again, one
-// read more.  The kernels are bound by HBM: 16,384 x 2,048 bf16 forward 46 us (5.8 TB/s), backward 66 us
-// (5.1 TB/s) and 4 us for dw's sum; 20,480 x 64 fp32 5 + 5 + 4 us.
+// read more.  The kernels are bound by HBM: 16,384 x 2,048 bf16 forward 44 us (6.1 TB/s), backward 65 us
+// (5.2 TB/s) and 5 us for dw's sum; 20,480 x 64 fp32 5 + 5 + 4 us.
 //
 // The backward's dw: a thread owns the same columns for every row that its group takes (rows in a
 // grid-stride order), adds them up in registers, groups and waves of a block are joined in a fixed
@@ -24,7 +24,7 @@ namespace {
 using fr::bf16_t;
 
 // upper limit of the backward's blocks = partial rows of dw: three per compute unit are resident with wide rows
-// (16,384 x 2,048 bf16: 51 us, 61 us with 1,024, whose last third waits)
+// (16,384 x 2,048 bf16 with a residual: 65 us, 73 us with 1,024, whose last third waits)
 constexpr int kBwdBlocks = 768;
 
 template <int G>
@@ -301,8 +301,9 @@ __global__ __launch_bounds__(256) void rms_dw_kernel(const float* __restrict__ p
   }
 }
 
-// G threads and K vectors per thread for `nv` vectors per row: the narrowest group that holds the row
-// in at most 8 vectors of one element or 4 of 16 bytes, a whole block where a wave does not
+// G threads and K vectors per thread for `nv` vectors per row: up to a wave with 1 to 4 vectors each, a whole block
+// with 2 to 8, and with 32 single elements for rows of more than 2,048 that are not whole 16-byte words (a row of
+// 2,049 keeps 32 slots per thread, too, three quarters of them empty)
 template <typename F>
 bool by_width(int64_t nv, F&& f) {
   if (nv <= 8) f(std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{});
