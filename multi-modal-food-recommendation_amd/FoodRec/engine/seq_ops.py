@@ -12,7 +12,8 @@ preference_loss(logp, ref, off)     bpr_emb_loss          paired log ratios of l
 Tables and rows are fp32 or bf16, arithmetic is fp32 (sums of a list's log-probabilities fp64; the matrix
 products of item_log_probs as it says), every stored value is rounded once.  All results are deterministic.  Calls are stream-ordered on the current
 stream of the tensors' device, never synchronise and may be captured into a HIP graph.  Each op is
-differentiable once, in reverse mode; forward-mode tangents and torch.jit.trace are refused.
+differentiable once, in reverse mode; forward-mode tangents, torch.jit.trace and torch.func's transforms are
+refused.
 
 The checks of arguments, the allocations and the autograd nodes are C++ (csrc/fr_torch.cpp): these ops
 are called singly on small batches, where a Python autograd function costs more than the kernel.

@@ -92,26 +92,28 @@ void plain_call(const char* name, const Tensor& t) {
   if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())
     fail(name, ": engine operators have no forward-mode derivative");
   if (torch::jit::tracer::isTracing()) fail(name, ": engine operators cannot be traced");
+  if (!t.has_storage()) fail(name, ": a dense tensor required (no sparse one, and none of torch.func's transforms)");
 }
 
 // the tensors on one GPU, the first in a supported type
 template <typename... O>
 void check(const char* name, const Tensor& t, const O&... others) {
-  plain_call(name, t);
-  on_gpu(t);
+  const auto plain = [&](const Tensor& o) { plain_call(name, o); };
   const auto same = [&](const Tensor& o) {
-    plain_call(name, o);
     on_gpu(o);
     if (o.device() != t.device()) fail(name, ": tensors on ", t.device(), " and ", o.device());
   };
-  const auto each = [&](const auto& o) {
+  const auto each = [&](const auto& o, const auto& f) {
     if constexpr (std::is_same_v<std::decay_t<decltype(o)>, MaybeTensor>) {
-      if (o) same(*o);
+      if (o) f(*o);
     } else {
-      same(o);
+      f(o);
     }
   };
-  (each(others), ...);
+  plain(t);
+  (each(others, plain), ...);
+  on_gpu(t);
+  (each(others, same), ...);
   if (t.scalar_type() != at::kFloat && t.scalar_type() != at::kBFloat16)
     fail(name, ": fp32 or bf16 tensors required (got ", t.scalar_type(), ")");
 }
