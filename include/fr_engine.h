@@ -1001,7 +1001,8 @@ int fr_rms_norm_bwd(const void* d_dy, int64_t lddy, const void* d_dh, int64_t ld
  * d_o [n, d] = sum_{v != ids[i]} p[i, v] W[v].  The table starts at a 16-byte boundary.  Masks by large negative
  * scores are taken at their value, up to the type's lowest (a row of nothing else is a uniform choice); scores beyond
  * +-2.3e38 (fp32's range in units of log 2) are that range's end.  A score of -inf is no choice (a row of nothing else
- * has NaN), and an infinite entry's column of dH no number (0 times it).
+ * has NaN), and an infinite entry's column of dH no number (0 times it).  d_o is summed before it is divided: items of
+ * weight whose entries are above 2^119 / n_items may overflow in their column (masked ones have no weight).
  * Precision: fp32 rows are multiplied in 16-bit parts that leave 2^-22 of a score's terms and 2^-23 of a score at most
  * (rows that differ too much for it go through fp32 instructions); bf16 rows exactly, with fp32 sums, which in dW are
  * added to the row's log-sum (rounded at its size), and probabilities that both gradients' products take in bf16 (the
